@@ -4,7 +4,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
-from ctypes import c_float, c_int, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_PKG, "csrc")
@@ -36,6 +36,15 @@ SIGNATURES = {
     "akv_decode_step_workspace_bytes": (c_size_t, [_I, _I, _I, _I]),
     "akv_decode_step": (c_int, [_P] * 14 + [_I] + [_P] * 3 + [_I, _P, c_size_t] + [_P] * 3 + [_I] * 12 + [_P]),
     "akv_decode_step_desc": (c_int, [_P] * 5 + [_I] + [_P] * 4 + [_I, _P, _I, _I, _P]),
+    "akv_prefill_attention_workspace_bytes": (c_size_t, [_I, _I]),
+    "akv_prefill_attention": (c_int, [_P, _P, _P, _I, _P, c_size_t, _P]),
+    "akv_attention_weights": (c_int, [_P, _P, _I, _P, c_int64, c_int64, _I, _P]),
+    "akv_accumulate_weights": (c_int, [_P, c_int64, c_int64, _P, _I, _P, _P, c_int64, c_int64, _I, _I, _I, _I, c_float, _P]),
+    "akv_tree_attention_workspace_bytes": (c_size_t, [_I] * 6),
+    "akv_tree_attention": (c_int, [_P] * 5 + [_I, _P, c_float, c_float, _P, _I, _I, _I, _P, c_size_t, _P]),
+    "akv_tree_commit": (c_int, [_P, _I, _P, _P, _P, _I, _I, _P]),
+    "akv_evict_workspace_bytes": (c_size_t, [_I] * 6),
+    "akv_evict": (c_int, [_P, _P, _P, c_int64, c_int64, _P, c_int64, c_int64, _I, _P, _I, _I, _I, _P, c_size_t, _P]),
     "akv_decode_step_static": (c_int, [_P] * 14 + [_I] + [_P] * 3 + [_I] + [_P] * 3 + [_I] * 12 + [_P]),
 }
 
@@ -47,6 +56,20 @@ class StepDesc(ctypes.Structure):
                 + [("workspace_bytes", c_size_t)]
                 + [(n, _I) for n in ("row_stride", "bsz", "n_q_heads", "n_kv_heads", "n_max_blocks", "max_seq_len", "head_dim",
                                      "d_block", "k_block", "top_max_k")])
+
+
+class PromptDesc(ctypes.Structure):
+    """akv_prompt_desc of include/alignedkv.h."""
+    _fields_ = ([(n, _P) for n in ("q", "k", "v")] + [(n, c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [(n, _P) for n in ("slopes", "seq_lens", "prefix_lens", "documents")]
+                + [(n, _I) for n in ("bsz", "seqlen", "n_q_heads", "n_kv_heads", "head_dim")] + [("scale", c_float), ("softcap", c_float)])
+
+
+class CacheLayer(ctypes.Structure):
+    """akv_cache_layer of include/alignedkv.h."""
+    _fields_ = ([(n, _P) for n in ("k_first_8", "k_mid_4", "k_last_4", "v_first_8", "v_mid_4", "v_last_4", "k_exp_column_max",
+                                   "v_exp_column_max", "restk", "restv", "seq_lens")]
+                + [(n, _I) for n in ("bsz", "n_kv_heads", "n_max_blocks", "max_seq_len", "head_dim", "k_block")])
 
 
 def build(verbose: bool = False) -> str:

@@ -1,0 +1,428 @@
+// Prompt attention, and the attention weight that prompt tokens received.
+//
+//   s_ij = cap(scale q_i . k_j) - slope_h |i - j|,   cap(x) = c tanh(x / c)
+//   o_i  = sum_j softmax_j(s_ij) v_j,   lse_i = log sum_j exp(s_ij)
+// over the tokens j that row i sees: i, j < length, j <= i or j < prefix, same document (ids >= 0).  A row that sees
+// nothing gives zeros and lse = -inf.
+#include "akv_attention.h"
+
+namespace akv {
+
+struct PromptArgs {
+    const uint8_t *q, *k, *v;                 // fp16
+    int64_t q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h;   // strides in bytes
+    const float *slopes;                      // [Hq] or null
+    const int *lens, *prefix;                 // [B] or null
+    const int *docs;                          // [B, S] or null
+    const u32x4 *doc_tiles;                   // [B, tiles] of 64 tokens: {smallest id, largest id, all the same, 0}
+    int B, S, Hq, Hkv, G;
+    ScoreForm form;
+    float neg_slope_unit;                     // -log2 e
+};
+
+constexpr int kTile = 64;       // tokens per K/V tile and per document range
+
+__global__ __launch_bounds__(256) void doc_tiles_kernel(const int *__restrict__ docs, const int *__restrict__ lens, u32x4 *__restrict__ out,
+                                                        int S, int tiles) {
+    const int b = blockIdx.y, t = blockIdx.x * 4 + wave_index(), lane = threadIdx.x & 63;
+    if (t >= tiles) return;
+    const int n = lens ? min(lens[b], S) : S;
+    const int j = t * kTile + lane;
+    const int d = j < n ? docs[(int64_t)b * S + j] : -1;
+    const bool real = d >= 0;
+    const u32 lo = wave_min_u32(real ? (u32)d : 0x7fffffffu);
+    const u32 hi = ~wave_min_u32(real ? ~(u32)d : 0xffffffffu);   // largest id; 0 where there is none (then lo > hi)
+    const bool same = __all(!(j < n) || (u32)d == lo) && lo <= hi;
+    if (lane == 0) out[(int64_t)b * tiles + t] = u32x4{lo, hi, same ? 1u : 0u, 0u};
+}
+
+// The K/V tiles a workgroup has to look at, in order.  Without documents all of [0, end); with them those whose range of
+// ids meets the rows' (64 ranges per look).
+template <bool DOCS>
+struct TileWalk {
+    const u32x4 *ranges = nullptr;
+    u32 lo = 0, hi = 0;
+    bool rows_same = false;
+    int end = 0, next_tile = 0, base = -64;
+    unsigned long long live = 0, same = 0;
+    bool cur_same = true;       // every visible pair of (rows, last returned tile) is of one document
+
+    __device__ __forceinline__ int next() {
+        if constexpr (!DOCS) {
+            return next_tile < end ? next_tile++ : -1;
+        } else {
+            while (live == 0) {
+                base += 64;
+                if (base >= end) return -1;
+                const int t = base + (int)(threadIdx.x & 63);
+                u32x4 r = {1u, 0u, 0u, 0u};
+                if (t < end) r = ranges[t];
+                live = __ballot(t < end && r.x <= hi && r.y >= lo && r.x <= r.y);
+                same = __ballot(r.z != 0 && rows_same && r.x == lo);
+            }
+            const int i = __builtin_ctzll(live);
+            live &= live - 1;
+            cur_same = (same >> i) & 1;
+            return base + i;
+        }
+    }
+};
+
+// A workgroup's share of the work: query tile, query head, sequence.  Blocks are dealt out to the 8 XCDs in turn; the
+// query heads of one KV head, which read the same keys and values, are kept on one XCD (its L2), and the tiles with the
+// most tokens to look at (the last ones, under a causal mask) come first.
+__device__ __forceinline__ void prompt_block(int id, int n_tiles, int B, int Hkv, int G, int &qt, int &hq, int &b) {
+    const int streams = B * Hkv;
+    int stream, rest;
+    if (streams % 8 == 0) {
+        const int per = streams / 8, x = id & 7, i = id >> 3;
+        stream = (i / G) % per * 8 + x;
+        rest = i / (G * per) * G + i % G;
+    } else {
+        stream = (id / G) % streams;
+        rest = id / (G * streams) * G + id % G;
+    }
+    qt = n_tiles - 1 - rest / G;
+    b = stream / Hkv;
+    hq = (stream - b * Hkv) * G + rest % G;
+}
+
+// grid n_tiles * Hq * B, 256 threads: 128 query rows of one head, 32 a wave.  K and V tiles of BN tokens go through
+// LDS, two buffers: the next tile's loads are in flight (in registers) while this one is computed.
+template <int D, int BN, bool CAP, bool ALIBI, bool DOCS>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptArgs a, uint8_t *__restrict__ out, float *__restrict__ lse,
+                                                                        int n_tiles, int fill) {
+    constexpr int CPR = D / 8;                       // 16-byte chunks of a token
+    constexpr int LPT = BN * CPR / 256;              // chunks a thread loads per tile and side
+    constexpr int TB = BN / 32;
+    constexpr int kSide = BN * D * 2;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kSide];
+    const int lane = threadIdx.x & 63, wave = wave_index(), half = lane >> 5;
+    int qt, hq, b;
+    prompt_block(blockIdx.x, n_tiles, a.B, a.Hkv, a.G, qt, hq, b);
+    const int hkv = hq / a.G;
+    const int n = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
+    const int prefix = a.prefix ? min(a.prefix[b], n) : 0;
+    const int row0 = qt * 128, i0 = row0 + wave * 32, i = i0 + (lane & 31);
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[cb][r] = 0.f;
+    RowState st;
+
+    if (row0 < n) {
+        f16x8 qf[D / 16];
+        const uint8_t *qp = a.q + b * a.q_b + (int64_t)min(i, n - 1) * a.q_s + hq * a.q_h;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const f16x8 *>(qp + (2 * ks + half) * 16);
+        const int my_doc = DOCS ? a.docs[(int64_t)b * a.S + min(i, n - 1)] : 0;
+        const float neg_slope = ALIBI ? a.slopes[hq] * -kLog2e : 0.f;
+        const int last_row = min(row0 + 127, n - 1);
+        TileWalk<DOCS> walk;
+        walk.end = (max(last_row + 1, prefix) + BN - 1) / BN;
+        if constexpr (DOCS) {
+            // BN == kTile: one range per tile
+            walk.ranges = a.doc_tiles + (int64_t)b * ((a.S + kTile - 1) / kTile);
+            const int t0 = row0 / kTile;
+            u32x4 r0 = walk.ranges[t0], r1 = r0;
+            if (t0 * kTile + kTile <= last_row) r1 = walk.ranges[t0 + 1];
+            walk.lo = min(r0.x, r1.x);
+            walk.hi = max(r0.x <= r0.y ? r0.y : 0u, r1.x <= r1.y ? r1.y : 0u);
+            walk.rows_same = r0.z && r1.z && r0.x == r1.x;
+        }
+        const uint8_t *kp = a.k + b * a.k_b + hkv * a.k_h, *vp = a.v + b * a.v_b + hkv * a.v_h;
+
+        u32x4 kr[LPT], vr[LPT];
+        auto request = [&](int t) {
+            const int j0 = t * BN, rows = min(BN, n - j0);
+            // rows behind the sequence's end are out of the descriptors' range: they read as zeros
+            const auto rk = make_rsrc(kp + (int64_t)j0 * a.k_s, (u32)((rows - 1) * a.k_s + D * 2));
+            const auto rv = make_rsrc(vp + (int64_t)j0 * a.v_s, (u32)((rows - 1) * a.v_s + D * 2));
+#pragma unroll
+            for (int c = 0; c < LPT; ++c) {
+                const int id = c * 256 + threadIdx.x, row = id / CPR, ch = id % CPR;
+                kr[c] = __builtin_amdgcn_raw_buffer_load_b128(rk, row < rows ? (int)(row * a.k_s) + ch * 16 : kSkip, 0, 0);
+                vr[c] = __builtin_amdgcn_raw_buffer_load_b128(rv, row < rows ? (int)(row * a.v_s) + ch * 16 : kSkip, 0, 0);
+            }
+        };
+        auto put = [&](int buf) {
+#pragma unroll
+            for (int c = 0; c < LPT; ++c) {
+                const int id = c * 256 + threadIdx.x, off = tile_byte<D>(id / CPR, id % CPR);
+                *reinterpret_cast<u32x4 *>(&lds[buf][0][off]) = kr[c];
+                *reinterpret_cast<u32x4 *>(&lds[buf][1][off]) = vr[c];
+            }
+        };
+        int t = walk.next();
+        bool same = walk.cur_same;
+        if (t >= 0) {
+            request(t);
+            put(0);
+        }
+        __syncthreads();
+        int buf = 0;
+        while (t >= 0) {
+            const int t_next = walk.next();
+            const bool same_next = walk.cur_same;
+            if (t_next >= 0) request(t_next);
+            const int j0 = t * BN;
+            const int wave_last = min(i0 + 31, n - 1);
+            if (i0 < n && (j0 <= wave_last || j0 < prefix)) {
+                const uint8_t *kt = lds[buf][0], *vt = lds[buf][1];
+                f32x16 x[TB];
+                tile_scores<D, BN>(x, kt, qf);
+                // token 32 tb + 8 (r / 4) + r % 4 of the tile is seen if that number is at most lim
+                const int lim = min(max(i, prefix - 1), n - 1) - j0 - 4 * half;
+                const bool masked = !(j0 + BN - 1 <= max(i0, prefix - 1) && j0 + BN <= n) || !same;
+                const float gap0 = (float)(j0 + 4 * half - i);
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        x[tb][r] = modified<CAP>(x[tb][r], a.form);
+                        if constexpr (ALIBI) x[tb][r] = fmaf(neg_slope, fabsf(gap0 + (float)(tb * 32 + 8 * (r >> 2) + (r & 3))), x[tb][r]);
+                    }
+                if (masked) {
+#pragma unroll
+                    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int c = tb * 32 + 8 * (r >> 2) + (r & 3);
+                            bool see = c <= lim;
+                            if constexpr (DOCS) {
+                                const int dj = a.docs[(int64_t)b * a.S + min(j0 + c + 4 * half, n - 1)];
+                                see = see && (same || (dj == my_doc && dj >= 0));
+                            }
+                            x[tb][r] = see ? x[tb][r] : kNegInf;
+                        }
+                }
+                f16x8 p[TB][2];
+                tile_softmax<D, BN>(x, st, o, p);
+                if (!masked) {
+                    tile_output<D, BN>(o, vt, p);
+                } else {
+                    tile_output_masked<D, BN>(o, vt, p, [&](int c) {
+                        bool see = c - 4 * half <= lim;
+                        if constexpr (DOCS) {
+                            const int dj = a.docs[(int64_t)b * a.S + min(j0 + c, n - 1)];
+                            see = see && (same || (dj == my_doc && dj >= 0));
+                        }
+                        return see;
+                    });
+                }
+            }
+            if (t_next >= 0) put(buf ^ 1);
+            __syncthreads();
+            buf ^= 1;
+            t = t_next;
+            same = same_next;
+        }
+    }
+
+    if (i >= a.S) return;
+    if (i >= n && !fill) return;
+    const float l = halves_sum(st.l);
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);    // (an undefined sum stays undefined)
+    uint8_t *op = out + (((int64_t)b * a.S + i) * a.Hq + hq) * (D * 2);
+    if (i >= n) {
+#pragma unroll
+        for (int c = 0; c < CPR / 2; ++c) *reinterpret_cast<u32x4 *>(op + (2 * c + half) * 16) = u32x4{0u, 0u, 0u, 0u};
+    } else {
+#pragma unroll
+        for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const u32x2 w = {pack_f16(o[cb][4 * g] * inv, o[cb][4 * g + 1] * inv), pack_f16(o[cb][4 * g + 2] * inv, o[cb][4 * g + 3] * inv)};
+                *reinterpret_cast<u32x2 *>(op + (cb * 32 + 8 * g + 4 * half) * 2) = w;
+            }
+    }
+    if (lse != nullptr && half == 0)
+        lse[((int64_t)b * a.Hq + hq) * a.S + i] = i < n ? (st.m == kNegInf ? kNegInf : (st.m + __builtin_amdgcn_logf(l)) * kLn2) : kNegInf;
+}
+
+// ---- the weight each token received -----------------------------------------------------------------------------------------------
+// w_j = sum over the heads g of the group and the rows i of the window of exp(s_ij - lse_i).  One wave owns 32 tokens of one
+// KV head: their keys stay in registers, the rows stream past them 32 at a time (q from L2: every wave of a KV head reads the
+// same rows), a lane sums its row's column of each product, and one reduction over the 32 rows ends it.  No atomics: the
+// sums' order is fixed.
+template <int D, bool CAP, bool ALIBI>
+__global__ __launch_bounds__(256) void attention_weights_kernel(PromptArgs a, const float *__restrict__ lse, int window, float *__restrict__ w,
+                                                                int64_t w_b, int64_t w_h, int add) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    const int hkv = blockIdx.y, b = blockIdx.z;
+    const int j0 = (blockIdx.x * 4 + wave_index()) * 32;
+    if (j0 >= a.S) return;
+    const int n = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
+    const int prefix = a.prefix ? min(a.prefix[b], n) : 0;
+    float sum[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+    if (j0 < n) {
+        f16x8 kf[D / 16];
+        const uint8_t *kp = a.k + b * a.k_b + (int64_t)min(j0 + col, n - 1) * a.k_s + hkv * a.k_h;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *reinterpret_cast<const f16x8 *>(kp + (2 * ks + half) * 16);
+        int doc[16];
+        if (a.docs) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) doc[r] = a.docs[(int64_t)b * a.S + min(j0 + 8 * (r >> 2) + 4 * half + (r & 3), n - 1)];
+        }
+        int first = window > 0 ? max(0, n - window) : 0;
+        if (j0 >= prefix) first = max(first, j0);       // rows before the tokens do not see them
+        for (int g = 0; g < a.G; ++g) {
+            const int hq = hkv * a.G + g;
+            const float neg_slope = ALIBI ? a.slopes[hq] * -kLog2e : 0.f;
+            for (int i0 = first; i0 < n; i0 += 32) {
+                const int i = i0 + col, ic = min(i, n - 1);
+                const uint8_t *qp = a.q + b * a.q_b + (int64_t)ic * a.q_s + hq * a.q_h;
+                const float row_lse = lse[((int64_t)b * a.Hq + hq) * a.S + ic];
+                f32x16 x;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], *reinterpret_cast<const f16x8 *>(qp + (2 * ks + half) * 16), x, 0, 0, 0);
+                const int lim = i < n ? min(max(i, prefix - 1), n - 1) - j0 - 4 * half : -1;
+                const int my_doc = a.docs ? a.docs[(int64_t)b * a.S + ic] : 0;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int c = 8 * (r >> 2) + (r & 3);
+                    // the difference is formed before it is brought to base 2: both terms may be far larger than it
+                    float d;
+                    if constexpr (CAP) d = fmaf(a.form.c1, tanh_f32(x[r] * a.form.c0), -row_lse);
+                    else d = fmaf(x[r], a.form.c0, -row_lse);
+                    if constexpr (ALIBI) d = fmaf(neg_slope * kLn2, fabsf((float)(j0 + 4 * half + c - i)), d);
+                    const bool see = c <= lim && (!a.docs || (doc[r] == my_doc && my_doc >= 0));
+                    sum[r] += see ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.f;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        float s = lane_group_sum<16>(sum[r]);
+        const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+        sum[r] = __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    }
+    if (col == 0) {
+        float *wp = w + b * w_b + hkv * w_h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = j0 + 8 * (r >> 2) + 4 * half + (r & 3);
+            if (j >= a.S) continue;
+            if (add) {
+                if (j < n) wp[j] += sum[r];
+            } else {
+                wp[j] = sum[r];
+            }
+        }
+    }
+}
+
+static int prompt_args(PromptArgs &a, const akv_prompt_desc *d, const char *what) {
+    AKV_REQUIRE(d != nullptr, "%s: null descriptor", what);
+    AKV_REQUIRE(d->q && d->k, "%s: null pointer", what);
+    AKV_REQUIRE(d->head_dim == 64 || d->head_dim == 128 || d->head_dim == 256, "%s: head_dim %d: 64, 128 or 256", what, d->head_dim);
+    AKV_REQUIRE(d->bsz >= 1 && d->seqlen >= 1 && d->seqlen <= (1 << 30) && d->n_kv_heads >= 1 && d->n_q_heads >= 1 && d->n_q_heads % d->n_kv_heads == 0,
+                "%s: bsz %d, seqlen %d, heads %d / %d", what, d->bsz, d->seqlen, d->n_q_heads, d->n_kv_heads);
+    AKV_REQUIRE(d->bsz <= 65535 && d->n_kv_heads <= 65535, "%s: at most 65535 sequences and KV heads", what);
+    AKV_REQUIRE(d->scale > 0.f && d->scale < 1e30f, "%s: scale %g must be positive and finite", what, d->scale);
+    AKV_REQUIRE(d->softcap >= 0.f && d->softcap < 1e30f, "%s: softcap %g must be zero (off) or positive and finite", what, d->softcap);
+    const int64_t *strides[3] = {d->q_stride, d->k_stride, d->v_stride};
+    const void *ptrs[3] = {d->q, d->k, d->v};
+    for (int t = 0; t < 3; ++t) {
+        if (ptrs[t] == nullptr) continue;
+        AKV_REQUIRE(((uintptr_t)ptrs[t] & 15) == 0, "%s: q, k and v must be 16-byte aligned", what);
+        for (int i = 0; i < 3; ++i)
+            AKV_REQUIRE(strides[t][i] >= 0 && strides[t][i] % 8 == 0, "%s: strides must be multiples of 8 elements and not negative", what);
+        AKV_REQUIRE(strides[t][1] < (1 << 24), "%s: a token stride of %lld elements: below 2^24", what, (long long)strides[t][1]);
+    }
+    a.q = d->q; a.k = d->k; a.v = d->v;
+    a.q_b = d->q_stride[0] * 2; a.q_s = d->q_stride[1] * 2; a.q_h = d->q_stride[2] * 2;
+    a.k_b = d->k_stride[0] * 2; a.k_s = d->k_stride[1] * 2; a.k_h = d->k_stride[2] * 2;
+    a.v_b = d->v_stride[0] * 2; a.v_s = d->v_stride[1] * 2; a.v_h = d->v_stride[2] * 2;
+    a.slopes = d->slopes; a.lens = d->seq_lens; a.prefix = d->prefix_lens; a.docs = d->documents;
+    a.doc_tiles = nullptr;
+    a.B = d->bsz; a.S = d->seqlen; a.Hq = d->n_q_heads; a.Hkv = d->n_kv_heads; a.G = d->n_q_heads / d->n_kv_heads;
+    a.form = score_form(d->scale, d->softcap);
+    return AKV_OK;
+}
+
+template <int D, int BN>
+static void launch_prefill(const PromptArgs &a, bool cap, uint8_t *out, float *lse, int fill, hipStream_t st) {
+    const int n_tiles = (a.S + 127) / 128;
+    const dim3 grid((u32)((int64_t)n_tiles * a.Hq * a.B));
+#define AKV_PREFILL(CAP, ALIBI, DOCS) \
+    hipLaunchKernelGGL((prefill_kernel<D, BN, CAP, ALIBI, DOCS>), grid, dim3(256), 0, st, a, out, lse, n_tiles, fill)
+    if (a.docs) {
+        if (cap) { if (a.slopes) AKV_PREFILL(true, true, true); else AKV_PREFILL(true, false, true); }
+        else { if (a.slopes) AKV_PREFILL(false, true, true); else AKV_PREFILL(false, false, true); }
+    } else {
+        if (cap) { if (a.slopes) AKV_PREFILL(true, true, false); else AKV_PREFILL(true, false, false); }
+        else { if (a.slopes) AKV_PREFILL(false, true, false); else AKV_PREFILL(false, false, false); }
+    }
+#undef AKV_PREFILL
+}
+
+}  // namespace akv
+
+extern "C" size_t akv_prefill_attention_workspace_bytes(int bsz, int seqlen) {
+    if (bsz < 1 || seqlen < 1) return 0;
+    return (size_t)bsz * ((seqlen + akv::kTile - 1) / akv::kTile) * sizeof(u32x4);
+}
+
+extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, float *lse, int fill_padding, void *workspace,
+                                     size_t workspace_bytes, akv_stream_t stream) {
+    akv::PromptArgs a;
+    const int rc = akv::prompt_args(a, desc, "prefill_attention");
+    if (rc != AKV_OK) return rc;
+    AKV_REQUIRE(a.v && out, "prefill_attention: null pointer");
+    AKV_REQUIRE(((uintptr_t)out & 15) == 0, "prefill_attention: out must be 16-byte aligned");
+    AKV_REQUIRE((int64_t)((a.S + 127) / 128) * a.Hq * a.B < (1ll << 31), "prefill_attention: too many rows");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.docs) {
+        const size_t need = akv_prefill_attention_workspace_bytes(a.B, a.S);
+        AKV_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
+                    "prefill_attention: documents need a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
+        const int tiles = (a.S + akv::kTile - 1) / akv::kTile;
+        a.doc_tiles = static_cast<const u32x4 *>(workspace);
+        hipLaunchKernelGGL(akv::doc_tiles_kernel, dim3((tiles + 3) / 4, a.B), dim3(256), 0, st, a.docs, a.lens, static_cast<u32x4 *>(workspace), a.S, tiles);
+    }
+    const bool cap = desc->softcap > 0.f;
+    if (desc->head_dim == 64) akv::launch_prefill<64, 64>(a, cap, out, lse, fill_padding, st);
+    else if (desc->head_dim == 128) akv::launch_prefill<128, 64>(a, cap, out, lse, fill_padding, st);
+    else akv::launch_prefill<256, 64>(a, cap, out, lse, fill_padding, st);
+    return akv::check_launch("prefill_attention");
+}
+
+extern "C" int akv_attention_weights(const akv_prompt_desc *desc, const float *lse, int window, float *weights, int64_t weights_stride_b,
+                                     int64_t weights_stride_h, int add, akv_stream_t stream) {
+    akv::PromptArgs a;
+    const int rc = akv::prompt_args(a, desc, "attention_weights");
+    if (rc != AKV_OK) return rc;
+    AKV_REQUIRE(lse && weights, "attention_weights: null pointer");
+    AKV_REQUIRE(window >= 0, "attention_weights: window %d must be 0 (every row) or positive", window);
+    AKV_REQUIRE(weights_stride_h >= a.S || a.Hkv == 1, "attention_weights: rows of %lld weights for %d tokens", (long long)weights_stride_h, a.S);
+    // differences against lse are formed in natural units
+    const bool cap = desc->softcap > 0.f;
+    a.form.c0 = cap ? desc->scale / desc->softcap : desc->scale;
+    a.form.c1 = desc->softcap;
+    const dim3 grid((a.S + 127) / 128, a.Hkv, a.B);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+#define AKV_WEIGHTS(D, CAP, ALIBI)                                                                                             \
+    hipLaunchKernelGGL((akv::attention_weights_kernel<D, CAP, ALIBI>), grid, dim3(256), 0, st, a, lse, window, weights, weights_stride_b, \
+                       weights_stride_h, add)
+#define AKV_WEIGHTS_D(D)                                                                                    \
+    do {                                                                                                    \
+        if (cap) { if (a.slopes) AKV_WEIGHTS(D, true, true); else AKV_WEIGHTS(D, true, false); }            \
+        else { if (a.slopes) AKV_WEIGHTS(D, false, true); else AKV_WEIGHTS(D, false, false); }              \
+    } while (0)
+    if (desc->head_dim == 64) AKV_WEIGHTS_D(64);
+    else if (desc->head_dim == 128) AKV_WEIGHTS_D(128);
+    else AKV_WEIGHTS_D(256);
+#undef AKV_WEIGHTS_D
+#undef AKV_WEIGHTS
+    return akv::check_launch("attention_weights");
+}

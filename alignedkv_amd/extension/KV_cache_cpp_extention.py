@@ -335,3 +335,5 @@ def _prepare_decode_step(self, k_planes, v_planes, k_exp_column_max, v_exp_colum
 _AlignedKVModule.prepare_decode_step = _prepare_decode_step
 
 cuda_module = _AlignedKVModule()
+
+from . import serving_ops as _serving_ops  # noqa: E402,F401  (adds its operators to the class)

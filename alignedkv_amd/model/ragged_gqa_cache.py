@@ -17,9 +17,11 @@ from ..extension.KV_cache_cpp_extention import cuda_module
 
 class RaggedGQACache:
     def __init__(self, n_layers: int, bsz: int, max_seq_len: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
-                 device="cuda", literal_colmax: bool = True, k_block: int = column_block):
+                 device="cuda", literal_colmax: bool = True, k_block: int = column_block, track_weights: bool = False):
         """k_block: tokens per block of the K planes (64, or 256 for head_dim 64 / 128 and 2 to 16 query heads per KV
-        head: a nibble row of a channel is then a whole 128-byte line)."""
+        head: a nibble row of a channel is then a whole 128-byte line).
+        track_weights: decode() and prefill_packed() accumulate in `weights` the attention each cached token received,
+        which is what evict() goes by."""
         assert n_q_heads % n_kv_heads == 0 and k_block in (column_block, 4 * column_block)
         self.n_layers, self.bsz, self.max_seq_len = n_layers, bsz, max_seq_len
         self.n_q_heads, self.n_kv_heads, self.head_dim = n_q_heads, n_kv_heads, head_dim
@@ -44,6 +46,11 @@ class RaggedGQACache:
         self.scores = torch.empty((B, n_q_heads, width), dtype=torch.half, device=device)
         self.probs = torch.empty((B, n_q_heads, width), dtype=torch.half, device=device)
         self.last_k_levels = self.last_v_levels = self.last_alignment_min = None
+        # fp32 [bsz, n_kv_heads, max_seq_len] per layer: summed probabilities, by the token's place in the cache
+        self.weights = [torch.zeros((B, H, max_seq_len), dtype=torch.float32, device=device) for _ in range(n_layers)] \
+            if track_weights else None
+        self._evicted = [[False] * B for _ in range(n_layers)]   # places are no longer positions
+        self._prepared = [None] * n_layers
 
     def _colmax(self, x: torch.Tensor) -> torch.Tensor:
         if self.literal_colmax:   # exponent of the signed maximum, as the reference's prefill computes it
@@ -71,6 +78,9 @@ class RaggedGQACache:
         self.restv[layer][b, :tail] = v[0, S - tail:]
         self.seq_lens[layer][b] = S
         self.len_bound[layer] = max(self.len_bound[layer], S)
+        self._evicted[layer][b] = False
+        if self.weights is not None:
+            self.weights[layer][b].zero_()
 
     def decode(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask2d=None, bound=None) -> torch.Tensor:
         """One decode step for every sequence: q fp16 [bsz,1,n_q_heads,head_dim], k/v [bsz,1,n_kv_heads,head_dim].
@@ -98,6 +108,8 @@ class RaggedGQACache:
                                     k_block=self.k_block)
         if not fixed_bound:
             self.len_bound[layer] = bound + 1
+        if self.weights is not None:
+            cuda_module.accumulate_weights(self.weights[layer], self.probs, self.seq_lens[layer])
         self.last_k_levels, self.last_v_levels, self.last_alignment_min = klv, vlv, amin
         return out
 
@@ -117,3 +129,79 @@ class RaggedGQACache:
         with torch.cuda.graph(graph):
             out = self.decode(layer, q, k, v, bound=self.max_seq_len - 1)
         return graph, q, k, v, out
+
+    # ---- whole prompts, drafted tokens, eviction ---------------------------------------------------------------------
+    def prepared(self, layer: int):
+        """The layer's descriptor for cuda_module.tree_attention / tree_commit / evict, made once (its tensors stay for the
+        cache's life)."""
+        if self._prepared[layer] is None:
+            self._prepared[layer] = cuda_module.prepare_layer(
+                self.k_planes[layer], self.v_planes[layer], self.k_colmax[layer], self.v_colmax[layer], self.restk[layer],
+                self.restv[layer], self.seq_lens[layer])
+        return self._prepared[layer]
+
+    def prefill_packed(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lens, *, scale=None, softcap: float = 0.0,
+                       slopes=None, window: int = 0) -> torch.Tensor:
+        """Attention of several prompts packed into one row, and their storage: sequence b takes the next lens[b] tokens.
+        q fp16 [1, sum(lens), n_q_heads, head_dim], k, v [1, sum(lens), n_kv_heads, head_dim]; lens: at most bsz positive
+        integers.  Returns fp16 [1, sum(lens), n_q_heads, head_dim].  Score form: cuda_module.prefill_attention.  With
+        track_weights the weights of these sequences start from the last `window` rows of each prompt (0: all rows)."""
+        lens = [int(n) for n in lens]
+        S = sum(lens)
+        assert 1 <= len(lens) <= self.bsz and min(lens) >= 1, f"lens {lens}: 1 to {self.bsz} prompts of at least one token"
+        assert max(lens) <= self.max_seq_len, "cache full"
+        assert tuple(q.shape) == (1, S, self.n_q_heads, self.head_dim) and tuple(k.shape) == (1, S, self.n_kv_heads, self.head_dim) \
+            and k.shape == v.shape
+        docs = None
+        if len(lens) > 1:
+            docs = torch.repeat_interleave(torch.arange(len(lens), dtype=torch.int32), torch.tensor(lens)).to(q.device)[None]
+        form = dict(scale=scale, softcap=softcap, slopes=slopes)
+        out, lse = cuda_module.prefill_attention(q, k, v, documents=docs, return_lse=True, **form)
+        start = 0
+        for b, n in enumerate(lens):
+            self.prefill(layer, b, k[:, start:start + n], v[:, start:start + n])
+            if self.weights is not None:
+                at = slice(start, start + n)
+                cuda_module.attention_weights(q[:, at], k[:, at], lse[:, :, at].contiguous(), window=window,
+                                              out=self.weights[layer][b:b + 1], **form)
+            start += n
+        return out
+
+    def verify(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ancestors=None, *, scale=None, softcap: float = 0.0,
+               slopes=None, bound=None) -> torch.Tensor:
+        """Attention of drafted tokens over the cache and each other: q fp16 [bsz, T, n_q_heads, head_dim], k, v
+        [bsz, T, n_kv_heads, head_dim], T at most 64; ancestors: cuda_module.tree_attention (default: a chain).  Returns fp16
+        [bsz, T, n_q_heads, head_dim].  Nothing is stored: commit() appends the drafts that were accepted.  bound: upper
+        bound of the lengths that sizes the launch (default: the largest length this object has seen)."""
+        if slopes is not None and any(self._evicted[layer]):
+            raise RuntimeError("verify: a distance bias needs the tokens' positions, which eviction does not keep")
+        bound = self.len_bound[layer] if bound is None else bound
+        return cuda_module.tree_attention(self.prepared(layer), q, k, v, ancestors, scale=scale, softcap=softcap, slopes=slopes, bound=bound)
+
+    def commit(self, k, v, accepted: torch.Tensor, layers=None, most=None):
+        """Appends the accepted drafts to `layers` (default: all): k, v: one tensor [bsz, T, n_kv_heads, head_dim] per layer (a
+        list, or stacked); accepted int32 [bsz, A] on the device: indices of drafts in order, -1 behind the last.  most: the
+        largest number of tokens any sequence accepted, if the host knows it (the length bound grows by A otherwise; see
+        refresh_bounds).  With track_weights the new tokens start at a weight of zero."""
+        layers = list(range(self.n_layers)) if layers is None else list(layers)
+        cuda_module.tree_commit([self.prepared(i) for i in layers], k, v, accepted)
+        for i in layers:
+            self.len_bound[i] = min(self.max_seq_len, self.len_bound[i] + (accepted.shape[1] if most is None else int(most)))
+
+    def refresh_bounds(self):
+        """Reads the lengths back (a synchronisation) and makes them the host-side bounds."""
+        for i, n in enumerate(self.seq_lens):
+            self.len_bound[i] = max(0, int(n.max()))
+
+    def evict(self, layer: int, keep: int, *, sinks: int = 0, recent: int = 0, into: "RaggedGQACache" = None) -> torch.Tensor:
+        """Keeps `keep` (a multiple of 64) of the tokens each sequence and KV head has in the planes (cuda_module.evict), by the
+        accumulated weights, in this cache or, as the same layer, in another one.  Returns the kept tokens' old places."""
+        if self.weights is None:
+            raise RuntimeError("evict: made without track_weights")
+        to = self if into is None else into
+        kept = cuda_module.evict(self.prepared(layer), self.weights[layer], keep, sinks=sinks, recent=recent,
+                                 into=None if into is None else into.prepared(layer),
+                                 into_weights=None if into is None or into.weights is None else into.weights[layer])
+        to.len_bound[layer] = min(self.len_bound[layer], keep + column_block - 1)
+        to._evicted[layer] = [True] * self.bsz
+        return kept

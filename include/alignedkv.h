@@ -233,6 +233,88 @@ AKV_API int akv_decode_step_desc(const akv_step_desc *desc, const uint8_t *q, co
                                  int flags, akv_stream_t stream);
 
 /*
+ * ---- Serving operators over the split-plane cache (no counterpart in the reference) ---------------------------------------
+ *
+ * A score is  s_ij = cap(scale * q_i . k_j) - slope_h * |pos_i - pos_j|  with cap(x) = softcap * tanh(x / softcap), or x where
+ * softcap is 0; slopes: fp32 [n_q_heads] or NULL (no distance bias).  Products are accumulated, and softmax statistics, sums and
+ * weights held, in 32 bits; probabilities are rounded to fp16 for the product with V, outputs once at the end.  A row that sees no
+ * token gives zeros.  A value that is infinite or not a number reaches exactly the rows that see its token.
+ */
+
+/* A batch of prompts.  q, k, v: fp16 [bsz, seqlen, heads, head_dim], innermost dense, strides in elements between batches, tokens
+ * and heads (multiples of 8, the token stride below 2^24; pointers 16-byte aligned); head_dim 64, 128 or 256; n_q_heads a
+ * multiple of n_kv_heads.  Row i sees token j if i, j < seq_lens[b], and j <= i or j < prefix_lens[b], and documents[b][i] ==
+ * documents[b][j] >= 0; seq_lens, prefix_lens int32 [bsz] and documents int32 [bsz, seqlen] are optional (NULL). */
+typedef struct akv_prompt_desc {
+    const uint8_t *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const float *slopes;
+    const int *seq_lens, *prefix_lens, *documents;
+    int bsz, seqlen, n_q_heads, n_kv_heads, head_dim;
+    float scale, softcap;
+} akv_prompt_desc;
+
+/* out: fp16 [bsz, seqlen, n_q_heads, head_dim] contiguous; lse (optional): fp32 [bsz, n_q_heads, seqlen], the logarithm of the row's sum
+ * (-inf for a row that sees nothing).  Rows at and beyond seq_lens are zeros / -inf if fill_padding, otherwise left as they were.
+ * workspace: needed with documents only. */
+AKV_API size_t akv_prefill_attention_workspace_bytes(int bsz, int seqlen);
+AKV_API int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, float *lse, int fill_padding, void *workspace,
+                                  size_t workspace_bytes, akv_stream_t stream);
+
+/* weights[b][h][j] (+)= sum over the query heads of KV head h and the last `window` rows i of sequence b (0: every row) of
+ * exp(s_ij - lse_i); desc->v is not read.  weights: fp32, innermost dense.  add = 0: all seqlen entries are written (zero beyond the
+ * length); add = 1: entries below the length are added to. */
+AKV_API int akv_attention_weights(const akv_prompt_desc *desc, const float *lse, int window, float *weights, int64_t weights_stride_b,
+                                  int64_t weights_stride_h, int add, akv_stream_t stream);
+
+/* out[b][h][t] = decay * weights[b][h][t] + sum over the query heads of KV head h of probs[b][.][t], t < min(seq_lens[b], capacity);
+ * other entries are left as they were.  probs: fp16 [bsz, n_q_heads, row_stride], what akv_decode_step* records (seq_lens as the
+ * step leaves them).  out may be weights. */
+AKV_API int akv_accumulate_weights(const float *weights, int64_t weights_stride_b, int64_t weights_stride_h, const uint8_t *probs,
+                                   int row_stride, const int *seq_lens, float *out, int64_t out_stride_b, int64_t out_stride_h, int bsz,
+                                   int n_q_heads, int n_kv_heads, int capacity, float decay, akv_stream_t stream);
+
+/* One layer of a cache with a length per sequence (the state akv_decode_step_gqa works on with seq_lens): planes, column maxima,
+ * fp16 rest buffers [bsz, 64, n_kv_heads, head_dim] and the lengths, int32 [bsz] on the device.  Sequence b holds seq_lens[b] tokens, the
+ * first seq_lens[b] / 64 * 64 of them in the planes.  head_dim 64, 128 or 256; k_block 64 or 256. */
+typedef struct akv_cache_layer {
+    uint8_t *k_first_8, *k_mid_4, *k_last_4, *v_first_8, *v_mid_4, *v_last_4;
+    uint8_t *k_exp_column_max, *v_exp_column_max, *restk, *restv;
+    int *seq_lens;
+    int bsz, n_kv_heads, n_max_blocks, max_seq_len, head_dim, k_block;
+} akv_cache_layer;
+
+/* Attention of n_drafts (1 to 64) drafted tokens per sequence over the whole cache, every plane read, and over the drafts in their
+ * masks: bit u of ancestors[t] (int64, [n_drafts], or [bsz, n_drafts] with ancestors_per_sequence) says that draft t sees draft u, itself
+ * included if bit t is set.  Draft t stands at position seq_lens[b] + (number of other drafts it sees).  q, out: fp16
+ * [bsz, n_drafts, n_q_heads, head_dim]; k, v: fp16 [bsz, n_drafts, n_kv_heads, head_dim].  len_bound: upper bound of the lengths
+ * (whole tiles of the planes beyond it are not looked at).  The cache is not changed.  One draft whose mask is its own bit is a decode step without
+ * fetch decisions. */
+AKV_API size_t akv_tree_attention_workspace_bytes(int bsz, int n_q_heads, int n_kv_heads, int head_dim, int n_drafts, int len_bound);
+AKV_API int akv_tree_attention(const akv_cache_layer *layer, const uint8_t *q, const uint8_t *k, const uint8_t *v, const int64_t *ancestors,
+                               int ancestors_per_sequence, const float *slopes, float scale, float softcap, uint8_t *out, int n_drafts,
+                               int n_q_heads, int len_bound, void *workspace, size_t workspace_bytes, akv_stream_t stream);
+
+/* Appends accepted drafts to the caches of n_layers layers of one shape: the drafts accepted[b][0 .. ] (int32 [bsz, n_accepted] on the
+ * device, n_accepted at most 64), up to the first entry outside [0, n_drafts), as that many decode steps would: column maxima, rest
+ * buffer, a flush of 64 tokens when it fills, lengths.  k[i], v[i]: layer i's fp16 [bsz, n_drafts, n_kv_heads, head_dim].  What does not fit
+ * into max_seq_len is dropped.  Rows of a rest buffer at and beyond its new count are left as they were. */
+AKV_API int akv_tree_commit(const akv_cache_layer *layers, int n_layers, const uint8_t *const *k, const uint8_t *const *v,
+                            const int *accepted, int n_drafts, int n_accepted, akv_stream_t stream);
+
+/* Keeps `keep` (a multiple of 64) of the tokens in the planes of each sequence and KV head: the first `sinks`, those among the newest
+ * `recent` tokens of the sequence, then the largest weights (ties: the lower index; not-a-number last), in their order at places 0 ..;
+ * all of them where there are no more than `keep`.  The rest buffer follows, so a sequence of n tokens is left with min(keep, n / 64 * 64)
+ * + n % 64.  kept: int32 [bsz, n_kv_heads, keep], the tokens' old places (-1 behind the last).  `to` is the same cache (its contents
+ * move; sequences that keep everything are not touched) or another of the same batch, heads, head_dim and k_block.  weights: fp32,
+ * as accumulated; weights_to (optional): the weights that move along, zeros up to its capacity behind them.  Column maxima are copied
+ * as they are (bounds of what is kept). */
+AKV_API size_t akv_evict_workspace_bytes(int bsz, int n_kv_heads, int head_dim, int k_block, int keep, int in_place);
+AKV_API int akv_evict(const akv_cache_layer *from, const akv_cache_layer *to, const float *weights, int64_t weights_stride_b,
+                      int64_t weights_stride_h, float *weights_to, int64_t to_stride_b, int64_t to_stride_h, int weights_to_capacity,
+                      int *kept, int keep, int sinks, int recent, void *workspace, size_t workspace_bytes, akv_stream_t stream);
+
+/*
  * Dense fp16 decode attention, the baseline of the benchmark (semantics of the reference's dense branch,
  * model/Llama_AlignedKV.py:130-139): appends k_new / v_new at row cur_len of the head-major fp16 caches
  * [bsz, heads, max_seq_len, head_dim] and attends over cur_len + 1 tokens.  q, k_new, v_new, out: fp16
