@@ -39,20 +39,22 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// tanh in 32 bits.  Near zero a series keeps the relative error at rounding level, where 1 - 2 / (exp(2 y) + 1) would
-// lose it to cancellation; a capped score is cap * tanh, so what is lost here is multiplied by the cap.
-// |y| < 1/2: odd polynomial through y^13 (Taylor coefficients; the first one left out is below 2e-8 relative there).
+// tanh in 32 bits.  |y| <= 0.6: an odd polynomial through y^9, fitted to tanh there (largest error 2.8e-8, below half a step of
+// tanh(0.6)); 1 - 2 / (exp(2 y) + 1) would lose small arguments to cancellation, and a capped score is cap * tanh, so what
+// is lost is multiplied by the cap.  Beyond: that form, from the hardware's 2^x and reciprocal.
+constexpr float kTanhNear = 0.6f;
+__device__ __forceinline__ float tanh_near(float y) {
+    const float z = y * y;
+    float p = fmaf(z, 0.015319169f, -0.051994310f);
+    p = fmaf(z, p, 0.13308098f);
+    p = fmaf(z, p, -0.33332248f);
+    return fmaf(y * z, p, y);
+}
 __device__ __forceinline__ float tanh_f32(float y) {
     const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
-    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-    const float z = y * y;
-    float p = fmaf(z, 21844.f / 6081075.f, -1382.f / 155925.f);
-    p = fmaf(z, p, 62.f / 2835.f);
-    p = fmaf(z, p, -17.f / 315.f);
-    p = fmaf(z, p, 2.f / 15.f);
-    p = fmaf(z, p, -1.f / 3.f);
-    const float near = fmaf(y * z, p, y);
-    return fabsf(y) < 0.4f ? near : far;
+    float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+    asm volatile("" : "+v"(far));      // both forms in straight code: a branch per score would cost more
+    return fabsf(y) <= kTanhNear ? tanh_near(y) : far;     // (not-a-number: far, which is not one either)
 }
 
 // What a raw product q . k goes through, in units of log2 e (so that the softmax takes 2^x):
@@ -71,6 +73,36 @@ __device__ __forceinline__ float modified(float raw, const ScoreForm &f) {
     if constexpr (CAP) return f.c1 * tanh_f32(raw * f.c0);
     return raw * f.c0;
 }
+// The same for a register block of a wave.  Capped scores are mostly far below their cap: where all of the wave's are within the
+// polynomial's range it alone is evaluated (7 instructions a score instead of 20, two of them at a quarter of the rate).
+template <bool CAP, int NB>
+__device__ __forceinline__ void modify_block(f32x16 (&x)[NB], const ScoreForm &f) {
+    if constexpr (CAP) {
+        float most = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[b][r]));
+        if (__all(most * f.c0 <= kTanhNear)) {      // (fmaxf passes over not-a-number; the polynomial hands it on)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[b][r] = f.c1 * tanh_near(x[b][r] * f.c0);
+                    if (r % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+                }
+            return;
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[b][r] = modified<CAP>(x[b][r], f);
+            if constexpr (CAP)
+                if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // (four at a time: all 32 at once need more registers than there are)
+        }
+}
 
 // ---- a tile of BN tokens x D channels in LDS, fp16, token-major ------------------------------------------------------------
 // 16-byte chunk c of row r lies at chunk c ^ swizzle(r): the lanes of one LDS access then spread over all banks, both for
@@ -85,58 +117,117 @@ __device__ __forceinline__ int tile_byte(int row, int chunk) {
     return row * (D * 2) + ((chunk ^ tile_swizzle<D>(row)) << 4);
 }
 
-typedef __attribute__((address_space(3))) const uint8_t *lds_ptr;
+// 16 bytes a lane from memory straight into LDS, lane l's at lds_base + 16 l (lds_base: the same in all lanes); nothing passes
+// through registers.  The compiler does not see these loads: wait_tile() before what they bring is read.
+__device__ __forceinline__ u32 lds_address(const void *p) { return (u32)(uintptr_t)(__attribute__((address_space(3))) const void *)p; }
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, u32 lds_base, int byte_off) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds_base)), "v"(byte_off), "s"(r)
+                 : "memory");
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// All of this wave's loads have arrived and its LDS reads are done, and so are the other waves'.
+__device__ __forceinline__ void wait_tile() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 typedef __attribute__((address_space(3))) s16x4 *lds_s16x4_ptr;
 
-// S^T of one tile: acc[tb] += K rows 32 tb .. 32 tb + 31 times the wave's 32 query rows.  qf[ks]: channels 16 ks + 8 half ..
+// Where a lane reads its operands in a tile: the part of the addresses that depends on the lane, so that what differs from read
+// to read is a constant (rows 16 apart lie alike) or one exclusive-or.
+template <int D>
+struct LaneBytes {
+    int k;                 // K operand, step 0; step ks: k ^ (ks << 5)
+    int v[2];              // V^T operand, channels 0 .. 31, first and second group of four tokens; block cb: v ^ (cb << 6)
+    __device__ __forceinline__ LaneBytes() {
+        const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+        k = tile_byte<D>(row, half);
+        const int vr = 4 * half + ((lane & 15) >> 2), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in_chunk = (lane & 1) * 8;
+        v[0] = tile_byte<D>(vr, chunk) + in_chunk;
+        v[1] = tile_byte<D>(vr + 8, chunk) + in_chunk;
+    }
+    // Once per tile: what is derived from these is worked out again (one instruction a read) instead of being kept in registers.
+    __device__ __forceinline__ void pin() { asm volatile("" : "+v"(k), "+v"(v[0]), "+v"(v[1])); }
+};
+
+// S^T of one tile: acc[tb] = K rows 32 tb .. 32 tb + 31 times the wave's 32 query rows.  qf[ks]: channels 16 ks + 8 half ..
 template <int D, int BN>
-__device__ __forceinline__ void tile_scores(f32x16 (&acc)[BN / 32], const uint8_t *k_tile, const f16x8 (&qf)[D / 16]) {
-    const int lane = threadIdx.x & 63, row = lane & 31, half = lane >> 5;
+__device__ __forceinline__ void tile_scores(f32x16 (&acc)[BN / 32], const uint8_t *k_tile, const LaneBytes<D> &at, const f16x8 (&qf)[D / 16]) {
 #pragma unroll
     for (int tb = 0; tb < BN / 32; ++tb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[tb][r] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-        const int off = tile_byte<D>(row, 2 * ks + half);
+        const uint8_t *kp = k_tile + (at.k ^ (ks << 5));
 #pragma unroll
-        for (int tb = 0; tb < BN / 32; ++tb) {
-            const f16x8 a = *reinterpret_cast<const f16x8 *>(k_tile + off + tb * 32 * D * 2);
-            acc[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[ks], acc[tb], 0, 0, 0);
-        }
+        for (int tb = 0; tb < BN / 32; ++tb)
+            acc[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const f16x8 *>(kp + tb * 32 * D * 2), qf[ks], acc[tb], 0, 0, 0);
+        if (ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);     // (operands of four steps in flight; all of them would not fit beside the sums)
     }
 }
 
 // The V^T operand for channels 32 cb .. + 31 and the 16 tokens whose probabilities are registers 8 s .. 8 s + 7 of block tb:
 // two transposing reads of four tokens each (lane group of 16: row r from the lanes 4 r .. 4 r + 3, column = lane).
 template <int D>
-__device__ __forceinline__ f16x8 tile_v_operand(const uint8_t *v_tile, int cb, int tb, int s) {
-    const int lane = threadIdx.x & 63;
-    const int row = tb * 32 + s * 16 + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int chunk = cb * 4 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in_chunk = (lane & 1) * 8;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(v_tile + tile_byte<D>(row, chunk) + in_chunk));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(v_tile + tile_byte<D>(row + 8, chunk) + in_chunk));
+__device__ __forceinline__ f16x8 tile_v_operand(const uint8_t *v_tile, const LaneBytes<D> &at, int cb, int tb, int s) {
+    const int rows = (tb * 32 + s * 16) * D * 2;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(v_tile + (at.v[0] ^ (cb << 6)) + rows));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(v_tile + (at.v[1] ^ (cb << 6)) + rows));
     return __builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// Any value of the operand infinite or not a number?
+// ---- infinite or undefined values in a V tile that some rows see only in part ----------------------------------------------------
+// A hidden token's probability is zero, but zero times such a value is undefined.  On a tile at the edge of what some row of the
+// workgroup sees, the waves look through the values first (a share each).  Where one is not finite (rare) what these values do
+// is noted apart: a row that sees +inf (or not-a-number) in a channel gets +inf added to its output there in the end, one that sees
+// -inf (or not-a-number) -inf; then they are zeroed in LDS and the tile goes the usual way.
+template <int D>
+struct OddValues {
+    u32 hit[2][D / 64] = {};      // [+inf, -inf]: bit 16 (cb % 2) + r of word cb / 2: this lane's row, channel of register r of block cb
+    __device__ __forceinline__ bool any() const {
+        u32 x = 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) x |= hit[s][i];
+        return __any(x != 0);
+    }
+    __device__ __forceinline__ void add(f32x16 (&o)[D / 32]) const {
+#pragma unroll
+        for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const u32 bit = 1u << (16 * (cb & 1) + r);
+                o[cb][r] += (hit[0][cb >> 1] & bit ? __builtin_inff() : 0.f) - (hit[1][cb >> 1] & bit ? __builtin_inff() : 0.f);
+            }
+    }
+};
+
+// This wave's share of the tile (4 waves): does it hold such a value?
+template <int D, int BN>
+__device__ __forceinline__ bool share_nonfinite(const uint8_t *v_tile) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int c = 0; c < BN * D / 2048; ++c) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(v_tile + (c * 256 + threadIdx.x) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
+    }
+    return __any(most.x >= 0x7C00 || most.y >= 0x7C00);
+}
 __device__ __forceinline__ bool any_nonfinite(f16x8 v) {
     const u32x4 w = __builtin_bit_cast(u32x4, v);
-    u32 bad = 0;
+    u32 hit = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const u32 e = w[i] & 0x7C007C00u;
-        bad |= ((e & 0xFFFFu) == 0x7C00u || (e >> 16) == 0x7C00u) ? 1u : 0u;
-    }
-    return bad != 0;
+    for (int i = 0; i < 4; ++i) hit |= ((w[i] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;    // (an exponent of all ones carries out)
+    return hit != 0;
 }
 __device__ __forceinline__ f16x8 zero_nonfinite(f16x8 v) {
     u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         u32 x = w[i];
-        if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u;
-        if ((x & 0x7C000000u) == 0x7C000000u) x &= 0x0000FFFFu;
+        x = (x & 0x7C00u) == 0x7C00u ? x & 0xFFFF0000u : x;
+        x = (x & 0x7C000000u) == 0x7C000000u ? x & 0x0000FFFFu : x;
         w[i] = x;
     }
     return __builtin_bit_cast(f16x8, w);
@@ -144,51 +235,52 @@ __device__ __forceinline__ f16x8 zero_nonfinite(f16x8 v) {
 
 // O^T += V^T P^T for one tile.  p[tb][s]: the probabilities as packed above.
 template <int D, int BN>
-__device__ __forceinline__ void tile_output(f32x16 (&o)[D / 32], const uint8_t *v_tile, const f16x8 (&p)[BN / 32][2]) {
+__device__ __forceinline__ void tile_output(f32x16 (&o)[D / 32], const uint8_t *v_tile, const LaneBytes<D> &at, const f16x8 (&p)[BN / 32][2]) {
 #pragma unroll
     for (int tb = 0; tb < BN / 32; ++tb)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int cb = 0; cb < D / 32; ++cb)
-                o[cb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(tile_v_operand<D>(v_tile, cb, tb, s), p[tb][s], o[cb], 0, 0, 0);
+                o[cb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(tile_v_operand<D>(v_tile, at, cb, tb, s), p[tb][s], o[cb], 0, 0, 0);
 }
 
-// The same where some rows do not see some tokens of the tile.  A hidden token's probability is zero, but zero times an
-// infinite or undefined value is undefined: such values are taken out of the product and added to the rows that do see
-// their token (which makes them infinite or undefined, as the formula does).  visible(t): does this lane's row see token t
-// of the tile?  Tiles without such values, the rule, pay one pass over the operands.
-template <int D, int BN, typename Visible>
-__device__ __forceinline__ void tile_output_masked(f32x16 (&o)[D / 32], const uint8_t *v_tile, const f16x8 (&p)[BN / 32][2],
-                                                   Visible visible) {
-    bool bad = false;
+// seen: bit 16 tb + r says that this lane's row sees the token of register r of block tb.
+template <int D, int BN>
+__device__ __forceinline__ void note_nonfinite(OddValues<D> &odd, const uint8_t *v_tile, const LaneBytes<D> &at, u32 seen) {
+    const u32 one = 0x3C00u;      // 1 in fp16
 #pragma unroll
-    for (int tb = 0; tb < BN / 32; ++tb)
+    for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int sign = 0; sign < 2; ++sign) {
+            f32x16 hits;          // how many +inf / -inf (not-a-number: both) each row sees in each channel
 #pragma unroll
-            for (int cb = 0; cb < D / 32; ++cb) {
-                f16x8 a = tile_v_operand<D>(v_tile, cb, tb, s);
-                if (any_nonfinite(a)) {
-                    bad = true;
-                    a = zero_nonfinite(a);
-                }
-                o[cb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[tb][s], o[cb], 0, 0, 0);
-            }
-    if (!__any(bad)) return;
-    const int half = (threadIdx.x & 63) >> 5;
+            for (int r = 0; r < 16; ++r) hits[r] = 0.f;
 #pragma unroll 1
-    for (int t = 0; t < BN; ++t) {
-        if (!visible(t)) continue;
+            for (int ts = 0; ts < BN / 16; ++ts) {
+                const u32x4 v = __builtin_bit_cast(u32x4, tile_v_operand<D>(v_tile, at, cb, ts >> 1, ts & 1));
+                u32x4 is, sees;
 #pragma unroll
-        for (int cb = 0; cb < D / 32; ++cb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int ch = cb * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-                const _Float16 v = *reinterpret_cast<const _Float16 *>(v_tile + tile_byte<D>(t, ch >> 3) + (ch & 7) * 2);
-                const float f = (float)v;
-                if (!(fabsf(f) < __builtin_inff())) o[cb][r] += f;
+                for (int i = 0; i < 4; ++i) {
+                    const u32 lo = v[i] & 0xFFFFu, hi = v[i] >> 16;
+                    const bool a = (lo & 0x7FFFu) > 0x7C00u || lo == (sign ? 0xFC00u : 0x7C00u), c = (hi & 0x7FFFu) > 0x7C00u || hi == (sign ? 0xFC00u : 0x7C00u);
+                    is[i] = (a ? one : 0u) | (c ? one << 16 : 0u);
+                    const u32 bits = seen >> (8 * ts + 2 * i);
+                    sees[i] = (bits & 1u ? one : 0u) | (bits & 2u ? one << 16 : 0u);
+                }
+                hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_f16x8(is), as_f16x8(sees), hits, 0, 0, 0);
             }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) odd.hit[sign][cb >> 1] |= hits[r] > 0.f ? 1u << (16 * (cb & 1) + r) : 0u;
+            asm volatile("" : "+v"(odd.hit[sign][cb >> 1]));      // now: not with the counts of all eight loops in registers
+        }
+}
+template <int D, int BN>
+__device__ __forceinline__ void zero_nonfinite_tile(uint8_t *v_tile) {
+#pragma unroll 1
+    for (int c = 0; c < BN * D / 2048; ++c) {
+        f16x8 *w = reinterpret_cast<f16x8 *>(v_tile + (c * 256 + threadIdx.x) * 16);
+        *w = zero_nonfinite(*w);
     }
 }
 

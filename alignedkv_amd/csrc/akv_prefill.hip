@@ -14,25 +14,26 @@ struct PromptArgs {
     const float *slopes;                      // [Hq] or null
     const int *lens, *prefix;                 // [B] or null
     const int *docs;                          // [B, S] or null
-    const u32x4 *doc_tiles;                   // [B, tiles] of 64 tokens: {smallest id, largest id, all the same, 0}
+    const u32x4 *doc_tiles;                   // [B, tiles of the K/V tile's tokens]: {smallest id, largest id, all the same, 0}
     int B, S, Hq, Hkv, G;
     ScoreForm form;
     float neg_slope_unit;                     // -log2 e
 };
 
-constexpr int kTile = 64;       // tokens per K/V tile and per document range
+constexpr int kTileMin = 32;    // tokens of a K/V tile, and of a range of documents: 64, or 32 for head_dim 256
 
 __global__ __launch_bounds__(256) void doc_tiles_kernel(const int *__restrict__ docs, const int *__restrict__ lens, u32x4 *__restrict__ out,
-                                                        int S, int tiles) {
+                                                        int S, int tiles, int tile) {
     const int b = blockIdx.y, t = blockIdx.x * 4 + wave_index(), lane = threadIdx.x & 63;
     if (t >= tiles) return;
     const int n = lens ? min(lens[b], S) : S;
-    const int j = t * kTile + lane;
-    const int d = j < n ? docs[(int64_t)b * S + j] : -1;
+    const int j = t * tile + lane;
+    const bool in = lane < tile && j < n;
+    const int d = in ? docs[(int64_t)b * S + j] : -1;
     const bool real = d >= 0;
     const u32 lo = wave_min_u32(real ? (u32)d : 0x7fffffffu);
     const u32 hi = ~wave_min_u32(real ? ~(u32)d : 0xffffffffu);   // largest id; 0 where there is none (then lo > hi)
-    const bool same = __all(!(j < n) || (u32)d == lo) && lo <= hi;
+    const bool same = __all(!in || (u32)d == lo) && lo <= hi;
     if (lane == 0) out[(int64_t)b * tiles + t] = u32x4{lo, hi, same ? 1u : 0u, 0u};
 }
 
@@ -87,8 +88,8 @@ __device__ __forceinline__ void prompt_block(int id, int n_tiles, int B, int Hkv
     hq = (stream - b * Hkv) * G + rest % G;
 }
 
-// grid n_tiles * Hq * B, 256 threads: 128 query rows of one head, 32 a wave.  K and V tiles of BN tokens go through
-// LDS, two buffers: the next tile's loads are in flight (in registers) while this one is computed.
+// grid n_tiles * Hq * B, 256 threads: 128 query rows of one head, 32 a wave.  K and V tiles of BN tokens go through LDS,
+// two buffers, filled by asynchronous loads: the next tile's are in flight while this one is computed, one barrier a tile.
 template <int D, int BN, bool CAP, bool ALIBI, bool DOCS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptArgs a, uint8_t *__restrict__ out, float *__restrict__ lse,
                                                                         int n_tiles, int fill) {
@@ -96,7 +97,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
     constexpr int LPT = BN * CPR / 256;              // chunks a thread loads per tile and side
     constexpr int TB = BN / 32;
     constexpr int kSide = BN * D * 2;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2][2][kSide];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][kSide];
+    __shared__ int odd_tile;                         // the last tile in which a wave found a value that is not finite
     const int lane = threadIdx.x & 63, wave = wave_index(), half = lane >> 5;
     int qt, hq, b;
     prompt_block(blockIdx.x, n_tiles, a.B, a.Hkv, a.G, qt, hq, b);
@@ -111,6 +113,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[cb][r] = 0.f;
     RowState st;
+    OddValues<D> odd;
 
     if (row0 < n) {
         f16x8 qf[D / 16];
@@ -123,98 +126,99 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
         TileWalk<DOCS> walk;
         walk.end = (max(last_row + 1, prefix) + BN - 1) / BN;
         if constexpr (DOCS) {
-            // BN == kTile: one range per tile
-            walk.ranges = a.doc_tiles + (int64_t)b * ((a.S + kTile - 1) / kTile);
-            const int t0 = row0 / kTile;
-            u32x4 r0 = walk.ranges[t0], r1 = r0;
-            if (t0 * kTile + kTile <= last_row) r1 = walk.ranges[t0 + 1];
-            walk.lo = min(r0.x, r1.x);
-            walk.hi = max(r0.x <= r0.y ? r0.y : 0u, r1.x <= r1.y ? r1.y : 0u);
-            walk.rows_same = r0.z && r1.z && r0.x == r1.x;
+            walk.ranges = a.doc_tiles + (int64_t)b * ((a.S + BN - 1) / BN);
+            walk.lo = 0xffffffffu;
+            walk.hi = 0;
+            walk.rows_same = true;
+            u32 first = 0;
+#pragma unroll
+            for (int s = 0; s < 128 / BN; ++s) {
+                if (row0 + s * BN > last_row) continue;
+                const u32x4 r = walk.ranges[row0 / BN + s];
+                if (s == 0) first = r.x;
+                walk.lo = min(walk.lo, r.x);
+                walk.hi = max(walk.hi, r.x <= r.y ? r.y : 0u);
+                walk.rows_same = walk.rows_same && r.z && r.x == first;
+            }
         }
         const uint8_t *kp = a.k + b * a.k_b + hkv * a.k_h, *vp = a.v + b * a.v_b + hkv * a.v_h;
-
-        u32x4 kr[LPT], vr[LPT];
-        auto request = [&](int t) {
+        // piece c * 256 + thread of a tile lies at that place in LDS: row piece / CPR, and the chunk that the layout puts there
+        const int my_row = threadIdx.x / CPR;
+        LaneBytes<D> at;
+        const u32 lds0 = lds_address(&lds[0][0][0]) + wave * 1024;
+        auto request = [&](int t, int buf) {
             const int j0 = t * BN, rows = min(BN, n - j0);
-            // rows behind the sequence's end are out of the descriptors' range: they read as zeros
             const auto rk = make_rsrc(kp + (int64_t)j0 * a.k_s, (u32)((rows - 1) * a.k_s + D * 2));
             const auto rv = make_rsrc(vp + (int64_t)j0 * a.v_s, (u32)((rows - 1) * a.v_s + D * 2));
 #pragma unroll
             for (int c = 0; c < LPT; ++c) {
-                const int id = c * 256 + threadIdx.x, row = id / CPR, ch = id % CPR;
-                kr[c] = __builtin_amdgcn_raw_buffer_load_b128(rk, row < rows ? (int)(row * a.k_s) + ch * 16 : kSkip, 0, 0);
-                vr[c] = __builtin_amdgcn_raw_buffer_load_b128(rv, row < rows ? (int)(row * a.v_s) + ch * 16 : kSkip, 0, 0);
+                // behind the sequence's end its last token stands in for the missing ones: no row sees them
+                const int r = my_row + c * (256 / CPR), row = min(r, rows - 1), ch = ((int)threadIdx.x % CPR ^ tile_swizzle<D>(r)) << 4;
+                load_to_lds(rk, lds0 + buf * (2 * kSide) + c * 4096, (int)(row * a.k_s) + ch);
+                load_to_lds(rv, lds0 + buf * (2 * kSide) + kSide + c * 4096, (int)(row * a.v_s) + ch);
             }
         };
-        auto put = [&](int buf) {
-#pragma unroll
-            for (int c = 0; c < LPT; ++c) {
-                const int id = c * 256 + threadIdx.x, off = tile_byte<D>(id / CPR, id % CPR);
-                *reinterpret_cast<u32x4 *>(&lds[buf][0][off]) = kr[c];
-                *reinterpret_cast<u32x4 *>(&lds[buf][1][off]) = vr[c];
-            }
-        };
-        int t = walk.next();
+        if (threadIdx.x == 0) odd_tile = -1;
+        int t = walk.next(), buf = 0;
         bool same = walk.cur_same;
-        if (t >= 0) {
-            request(t);
-            put(0);
-        }
-        __syncthreads();
-        int buf = 0;
+        if (t >= 0) request(t, 0);
         while (t >= 0) {
             const int t_next = walk.next();
             const bool same_next = walk.cur_same;
-            if (t_next >= 0) request(t_next);
+            wait_tile();
+            if (t_next >= 0) request(t_next, buf ^ 1);
             const int j0 = t * BN;
+            uint8_t *kt = lds[buf][0], *vt = lds[buf][1];
+            at.pin();
+            // token 32 tb + 8 (r / 4) + r % 4 of the tile is seen if that number is at most lim
+            const int lim = min(max(i, prefix - 1), n - 1) - j0 - 4 * half;
+            const bool whole = j0 + BN <= n && same;      // no row misses tokens for their length or document
+            int token_doc = 0;                             // of token `lane` of the tile
+            if constexpr (DOCS)
+                if (!same) token_doc = a.docs[(int64_t)b * a.S + min(j0 + lane, n - 1)];
+            const auto sees = [&](int c) {
+                bool see = c <= lim;
+                if constexpr (DOCS) {
+                    const int d0 = __builtin_amdgcn_readlane(token_doc, c), d1 = __builtin_amdgcn_readlane(token_doc, c + 4);
+                    see = see && (same || ((half ? d1 : d0) == my_doc && my_doc >= 0));
+                }
+                return see;
+            };
+            if (!whole || j0 + BN - 1 > max(row0, prefix - 1)) {
+                if (share_nonfinite<D, BN>(vt)) odd_tile = t;
+                lds_barrier();
+                if (odd_tile == t) {
+                    u32 seen = 0;
+#pragma unroll
+                    for (int c = 0; c < TB * 16; ++c) seen |= sees((c >> 4) * 32 + 8 * ((c & 15) >> 2) + (c & 3)) ? 1u << c : 0u;
+                    note_nonfinite<D, BN>(odd, vt, at, seen);
+                    lds_barrier();
+                    zero_nonfinite_tile<D, BN>(vt);
+                    lds_barrier();
+                }
+            }
             const int wave_last = min(i0 + 31, n - 1);
             if (i0 < n && (j0 <= wave_last || j0 < prefix)) {
-                const uint8_t *kt = lds[buf][0], *vt = lds[buf][1];
                 f32x16 x[TB];
-                tile_scores<D, BN>(x, kt, qf);
-                // token 32 tb + 8 (r / 4) + r % 4 of the tile is seen if that number is at most lim
-                const int lim = min(max(i, prefix - 1), n - 1) - j0 - 4 * half;
-                const bool masked = !(j0 + BN - 1 <= max(i0, prefix - 1) && j0 + BN <= n) || !same;
-                const float gap0 = (float)(j0 + 4 * half - i);
-#pragma unroll
-                for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        x[tb][r] = modified<CAP>(x[tb][r], a.form);
-                        if constexpr (ALIBI) x[tb][r] = fmaf(neg_slope, fabsf(gap0 + (float)(tb * 32 + 8 * (r >> 2) + (r & 3))), x[tb][r]);
-                    }
-                if (masked) {
+                tile_scores<D, BN>(x, kt, at, qf);
+                modify_block<CAP, TB>(x, a.form);
+                if constexpr (ALIBI) {
+                    const float gap0 = (float)(j0 + 4 * half - i);
 #pragma unroll
                     for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int c = tb * 32 + 8 * (r >> 2) + (r & 3);
-                            bool see = c <= lim;
-                            if constexpr (DOCS) {
-                                const int dj = a.docs[(int64_t)b * a.S + min(j0 + c + 4 * half, n - 1)];
-                                see = see && (same || (dj == my_doc && dj >= 0));
-                            }
-                            x[tb][r] = see ? x[tb][r] : kNegInf;
-                        }
+                        for (int r = 0; r < 16; ++r) x[tb][r] = fmaf(neg_slope, fabsf(gap0 + (float)(tb * 32 + 8 * (r >> 2) + (r & 3))), x[tb][r]);
+                }
+                if (!whole || j0 + BN - 1 > max(i0, prefix - 1)) {
+#pragma unroll
+                    for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[tb][r] = sees(tb * 32 + 8 * (r >> 2) + (r & 3)) ? x[tb][r] : kNegInf;
                 }
                 f16x8 p[TB][2];
                 tile_softmax<D, BN>(x, st, o, p);
-                if (!masked) {
-                    tile_output<D, BN>(o, vt, p);
-                } else {
-                    tile_output_masked<D, BN>(o, vt, p, [&](int c) {
-                        bool see = c - 4 * half <= lim;
-                        if constexpr (DOCS) {
-                            const int dj = a.docs[(int64_t)b * a.S + min(j0 + c, n - 1)];
-                            see = see && (same || (dj == my_doc && dj >= 0));
-                        }
-                        return see;
-                    });
-                }
+                tile_output<D, BN>(o, vt, at, p);
             }
-            if (t_next >= 0) put(buf ^ 1);
-            __syncthreads();
             buf ^= 1;
             t = t_next;
             same = same_next;
@@ -230,6 +234,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
 #pragma unroll
         for (int c = 0; c < CPR / 2; ++c) *reinterpret_cast<u32x4 *>(op + (2 * c + half) * 16) = u32x4{0u, 0u, 0u, 0u};
     } else {
+        if (odd.any()) odd.add(o);
 #pragma unroll
         for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
@@ -370,7 +375,7 @@ static void launch_prefill(const PromptArgs &a, bool cap, uint8_t *out, float *l
 
 extern "C" size_t akv_prefill_attention_workspace_bytes(int bsz, int seqlen) {
     if (bsz < 1 || seqlen < 1) return 0;
-    return (size_t)bsz * ((seqlen + akv::kTile - 1) / akv::kTile) * sizeof(u32x4);
+    return (size_t)bsz * ((seqlen + akv::kTileMin - 1) / akv::kTileMin) * sizeof(u32x4);
 }
 
 extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, float *lse, int fill_padding, void *workspace,
@@ -386,14 +391,14 @@ extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, 
         const size_t need = akv_prefill_attention_workspace_bytes(a.B, a.S);
         AKV_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                     "prefill_attention: documents need a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
-        const int tiles = (a.S + akv::kTile - 1) / akv::kTile;
+        const int tile = desc->head_dim == 256 ? 32 : 64, tiles = (a.S + tile - 1) / tile;
         a.doc_tiles = static_cast<const u32x4 *>(workspace);
-        hipLaunchKernelGGL(akv::doc_tiles_kernel, dim3((tiles + 3) / 4, a.B), dim3(256), 0, st, a.docs, a.lens, static_cast<u32x4 *>(workspace), a.S, tiles);
+        hipLaunchKernelGGL(akv::doc_tiles_kernel, dim3((tiles + 3) / 4, a.B), dim3(256), 0, st, a.docs, a.lens, static_cast<u32x4 *>(workspace), a.S, tiles, tile);
     }
     const bool cap = desc->softcap > 0.f;
     if (desc->head_dim == 64) akv::launch_prefill<64, 64>(a, cap, out, lse, fill_padding, st);
     else if (desc->head_dim == 128) akv::launch_prefill<128, 64>(a, cap, out, lse, fill_padding, st);
-    else akv::launch_prefill<256, 64>(a, cap, out, lse, fill_padding, st);
+    else akv::launch_prefill<256, 32>(a, cap, out, lse, fill_padding, st);
     return akv::check_launch("prefill_attention");
 }
 

@@ -295,11 +295,8 @@ __device__ __forceinline__ void tail_tile(const TreeArgs &a, Rows<D, NT> &s, int
         transpose8(in, op);
 #pragma unroll
         for (int c = 0; c < (CPL < 8 ? CPL : 8); ++c) {
-            f16x8 w = operand(op[c]);
-            if (any_nonfinite(w)) {
-                bad = true;
-                w = zero_nonfinite(w);
-            }
+            bad |= any_nonfinite(operand(op[c]));
+            const f16x8 w = zero_nonfinite(operand(op[c]));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 s.o[nt][8 * g + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, operand(p[nt]), s.o[nt][8 * g + c], 0, 0, 0);
