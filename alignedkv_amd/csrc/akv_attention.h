@@ -61,11 +61,18 @@ __device__ __forceinline__ float tanh_f32(float y) {
 //   no cap: x = raw * c0;  cap: x = c1 * tanh(raw * c0);  then x -= slope * |distance|.
 struct ScoreForm {
     float c0, c1;
+    float near, n1, n2, n3;      // |raw| <= near: x = c1 c0 raw (1 + n1 raw^2 + n2 raw^4 + n3 raw^6)
 };
 __host__ __device__ __forceinline__ ScoreForm score_form(float scale, float cap) {
-    ScoreForm f;
-    f.c0 = cap > 0.f ? scale / cap : scale * kLog2e;
-    f.c1 = cap * kLog2e;
+    ScoreForm f = {scale * kLog2e, 1.f, -1.f, 0.f, 0.f, 0.f};
+    if (cap > 0.f) {
+        f.c0 = scale / cap;
+        f.c1 = cap * kLog2e;
+        // an odd polynomial through the seventh power, fitted to tanh on |y| <= 0.4 (largest error 2.8e-8, half a step of tanh there), its
+        // coefficients for raw instead of y = raw * c0; powers that fp32 does not hold: no such range
+        const float z = f.c0 * f.c0;
+        if (f.c0 > 1e-5f && f.c0 < 1e5f) f = {f.c0, f.c1, 0.4f / f.c0, -0.333313877f * z, 0.132687496f * z * z, -0.0474229918f * z * z * z};
+    }
     return f;
 }
 template <bool CAP>
@@ -73,35 +80,36 @@ __device__ __forceinline__ float modified(float raw, const ScoreForm &f) {
     if constexpr (CAP) return f.c1 * tanh_f32(raw * f.c0);
     return raw * f.c0;
 }
-// The same for a register block of a wave.  Capped scores are mostly far below their cap: where all of the wave's are within the
-// polynomial's range it alone is evaluated (7 instructions a score instead of 20, two of them at a quarter of the rate).
+// The same for a register block of a wave, up to the factor that is returned (a softmax multiplies it in where it subtracts the
+// maximum).  Capped scores are mostly far below their cap: where all of the wave's are, the polynomial alone is evaluated (5
+// instructions a score instead of 20, two of them at a quarter of the rate).
 template <bool CAP, int NB>
-__device__ __forceinline__ void modify_block(f32x16 (&x)[NB], const ScoreForm &f) {
-    if constexpr (CAP) {
-        float most = 0.f;
+__device__ __forceinline__ float modify_block(f32x16 (&x)[NB], const ScoreForm &f) {
+    if constexpr (!CAP) return f.c0;
+    float most = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[b][r]));
+    if (__all(most <= f.near)) {      // (fmaxf passes over not-a-number; the polynomial hands it on)
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[b][r]));
-        if (__all(most * f.c0 <= kTanhNear)) {      // (fmaxf passes over not-a-number; the polynomial hands it on)
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    x[b][r] = f.c1 * tanh_near(x[b][r] * f.c0);
-                    if (r % 8 == 7) __builtin_amdgcn_sched_barrier(0);
-                }
-            return;
-        }
+            for (int r = 0; r < 16; ++r) {
+                const float z = x[b][r] * x[b][r];
+                x[b][r] *= fmaf(z, fmaf(z, fmaf(z, f.n3, f.n2), f.n1), 1.f);
+                if (r % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+            }
+        return f.c0 * f.c1;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            x[b][r] = modified<CAP>(x[b][r], f);
-            if constexpr (CAP)
-                if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // (four at a time: all 32 at once need more registers than there are)
+            x[b][r] = tanh_f32(x[b][r] * f.c0);
+            if (r % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // (four at a time: all 32 at once need more registers than there are)
         }
+    return f.c1;
 }
 
 // ---- a tile of BN tokens x D channels in LDS, fp16, token-major ------------------------------------------------------------
@@ -290,17 +298,17 @@ struct RowState {
     float l = 0.f;       // this lane's share of the sum
 };
 
-// x[tb][r] (units of log2 e, -inf where hidden) -> packed probabilities 2^(x - m); rescales l and o when the maximum grew
+// x[tb][r] (times factor > 0: units of log2 e; -inf where hidden) -> packed probabilities 2^(factor x - m); rescales l and o when the maximum grew
 // by more than 8 (a probability is then at most 2^8: far from fp16's limit, and sums keep their relative precision), which
 // after the first tiles of a row is rare.
 template <int D, int BN>
-__device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], RowState &st, f32x16 (&o)[D / 32], f16x8 (&p)[BN / 32][2]) {
+__device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], float factor, RowState &st, f32x16 (&o)[D / 32], f16x8 (&p)[BN / 32][2]) {
     float mx = x[0][0];
 #pragma unroll
     for (int tb = 0; tb < BN / 32; ++tb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[tb][r]);
-    mx = halves_max(mx);
+    mx = halves_max(mx) * factor;
     if (__any(mx > st.m + 8.f)) {     // (m = -inf: any finite maximum)
         const float m_new = fmaxf(st.m, mx);
         const float alpha = st.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(st.m - m_new);
@@ -317,7 +325,7 @@ __device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], RowState &st,
     for (int tb = 0; tb < BN / 32; ++tb) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            x[tb][r] = __builtin_amdgcn_exp2f(x[tb][r] - m);
+            x[tb][r] = __builtin_amdgcn_exp2f(fmaf(x[tb][r], factor, -m));
             sum += x[tb][r];
         }
 #pragma unroll
