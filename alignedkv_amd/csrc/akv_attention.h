@@ -209,14 +209,14 @@ struct OddValues {
     }
 };
 
-// This wave's share of the tile (4 waves): does it hold such a value?
-template <int D, int BN>
-__device__ __forceinline__ bool share_nonfinite(const uint8_t *v_tile) {
+// This wave's share of the tile (THREADS threads look through it, this is number tid): does it hold such a value?
+template <int D, int BN, int THREADS>
+__device__ __forceinline__ bool share_nonfinite(const uint8_t *v_tile, int tid) {
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     u16x2 most = {0, 0};
 #pragma unroll
-    for (int c = 0; c < BN * D / 2048; ++c) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(v_tile + (c * 256 + threadIdx.x) * 16);
+    for (int c = 0; c < BN * D / (8 * THREADS); ++c) {
+        const u32x4 w = *reinterpret_cast<const u32x4 *>(v_tile + (c * THREADS + tid) * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
     }
@@ -283,11 +283,11 @@ __device__ __forceinline__ void note_nonfinite(OddValues<D> &odd, const uint8_t 
             asm volatile("" : "+v"(odd.hit[sign][cb >> 1]));      // now: not with the counts of all eight loops in registers
         }
 }
-template <int D, int BN>
-__device__ __forceinline__ void zero_nonfinite_tile(uint8_t *v_tile) {
+template <int D, int BN, int THREADS>
+__device__ __forceinline__ void zero_nonfinite_tile(uint8_t *v_tile, int tid) {
 #pragma unroll 1
-    for (int c = 0; c < BN * D / 2048; ++c) {
-        f16x8 *w = reinterpret_cast<f16x8 *>(v_tile + (c * 256 + threadIdx.x) * 16);
+    for (int c = 0; c < BN * D / (8 * THREADS); ++c) {
+        f16x8 *w = reinterpret_cast<f16x8 *>(v_tile + (c * THREADS + tid) * 16);
         *w = zero_nonfinite(*w);
     }
 }
@@ -298,17 +298,17 @@ struct RowState {
     float l = 0.f;       // this lane's share of the sum
 };
 
-// x[tb][r] (times factor > 0: units of log2 e; -inf where hidden) -> packed probabilities 2^(factor x - m); rescales l and o when the maximum grew
+// Scores factor * x[tb][r] + shift (factor > 0; units of log2 e; x -inf where hidden) -> packed probabilities 2^(score - m); rescales l and o when the maximum grew
 // by more than 8 (a probability is then at most 2^8: far from fp16's limit, and sums keep their relative precision), which
 // after the first tiles of a row is rare.
 template <int D, int BN>
-__device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], float factor, RowState &st, f32x16 (&o)[D / 32], f16x8 (&p)[BN / 32][2]) {
+__device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], float factor, float shift, RowState &st, f32x16 (&o)[D / 32], f16x8 (&p)[BN / 32][2]) {
     float mx = x[0][0];
 #pragma unroll
     for (int tb = 0; tb < BN / 32; ++tb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[tb][r]);
-    mx = halves_max(mx) * factor;
+    mx = halves_max(fmaf(mx, factor, shift));
     if (__any(mx > st.m + 8.f)) {     // (m = -inf: any finite maximum)
         const float m_new = fmaxf(st.m, mx);
         const float alpha = st.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(st.m - m_new);
@@ -319,13 +319,13 @@ __device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], float factor,
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[cb][r] *= alpha;
     }
-    const float m = st.m == kNegInf ? 0.f : st.m;
+    const float less = shift - (st.m == kNegInf ? 0.f : st.m);
     float sum = 0.f;
 #pragma unroll
     for (int tb = 0; tb < BN / 32; ++tb) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            x[tb][r] = __builtin_amdgcn_exp2f(fmaf(x[tb][r], factor, -m));
+            x[tb][r] = __builtin_amdgcn_exp2f(fmaf(x[tb][r], factor, less));
             sum += x[tb][r];
         }
 #pragma unroll

@@ -130,25 +130,28 @@ __device__ __forceinline__ void prompt_block(int id, int n_tiles, int B, int Hkv
     hq = (stream - b * Hkv) * G + rest % G;
 }
 
-// grid n_tiles * Hq * B, 256 threads: 128 query rows of one head, 32 a wave.  K and V tiles of BN tokens go through LDS,
-// two buffers, filled by asynchronous loads: the next tile's are in flight while this one is computed, one barrier a tile.
-template <int D, int BN, bool CAP, bool ALIBI, bool DOCS>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptArgs a, uint8_t *__restrict__ out, float *__restrict__ lse,
-                                                                        int n_tiles, int fill) {
+// grid n_tiles * Hq * B, 256 threads.  K and V tiles of BN tokens go through LDS, two buffers, filled by asynchronous loads: the
+// next tiles are in flight while these are computed, one barrier a round.  PARTS == 1: 128 query rows of one head, 32 a wave, all
+// on the same tile.  PARTS == 2: 64 rows, two waves on every other tile each, their sums joined at the end: half the rounds for a
+// row, for calls whose longest rows, not their number, decide how long they take.
+template <int D, int BN, int PARTS, bool CAP, bool ALIBI, bool DOCS>
+__global__ __launch_bounds__(256, D == 256 || D * PARTS == 256 ? 1 : (D == 64 && PARTS == 1 && !DOCS ? 3 : 2)) void prefill_kernel(PromptArgs a, uint8_t *__restrict__ out, float *__restrict__ lse,
+                                                                                            int n_tiles, int fill) {
     constexpr int CPR = D / 8;                       // 16-byte chunks of a token
     constexpr int LPT = BN * CPR / 256;              // chunks a thread loads per tile and side
     constexpr int TB = BN / 32;
     constexpr int kSide = BN * D * 2;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2][kSide];
-    __shared__ int odd_tile;                         // the last tile in which a wave found a value that is not finite
-    const int lane = threadIdx.x & 63, wave = wave_index(), half = lane >> 5;
+    constexpr int ROWS = 128 / PARTS, WAVES = 4 / PARTS;      // rows of the workgroup, waves per part
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][PARTS][2][kSide];
+    __shared__ int odd_tile[PARTS];                  // the last tile in which a wave found a value that is not finite
+    const int lane = threadIdx.x & 63, wave = wave_index(), half = lane >> 5, part = wave / WAVES, tid = threadIdx.x & (64 * WAVES - 1);
     int qt, hq, b;
     prompt_block(blockIdx.x, n_tiles, a.B, a.Hkv, a.G, qt, hq, b);
     const int hkv = hq / a.G;
     if constexpr (DOCS) qt = a.order[(int64_t)b * n_tiles + n_tiles - 1 - qt];
     const int n = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
     const int prefix = a.prefix ? min(a.prefix[b], n) : 0;
-    const int row0 = qt * 128, i0 = row0 + wave * 32, i = i0 + (lane & 31);
+    const int row0 = qt * ROWS, i0 = row0 + (wave % WAVES) * 32, i = i0 + (lane & 31);
 
     f32x16 o[D / 32];
 #pragma unroll
@@ -165,7 +168,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
         for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const f16x8 *>(qp + (2 * ks + half) * 16);
         const int my_doc = DOCS ? a.docs[(int64_t)b * a.S + min(i, n - 1)] : 0;
         const float neg_slope = ALIBI ? a.slopes[hq] * -kLog2e : 0.f;
-        const int last_row = min(row0 + 127, n - 1);
+        const int last_row = min(row0 + ROWS - 1, n - 1);
         TileWalk<DOCS> walk;
         walk.end = (max(last_row + 1, prefix) + BN - 1) / BN;
         if constexpr (DOCS) {
@@ -175,7 +178,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
             walk.rows_same = true;
             u32 first = 0;
 #pragma unroll
-            for (int s = 0; s < 128 / BN; ++s) {
+            for (int s = 0; s < ROWS / BN; ++s) {
                 if (row0 + s * BN > last_row) continue;
                 const u32x4 r = walk.ranges[row0 / BN + s];
                 if (s == 0) first = r.x;
@@ -188,8 +191,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
         // piece c * 256 + thread of a tile lies at that place in LDS: row piece / CPR, and the chunk that the layout puts there
         const int my_row = threadIdx.x / CPR;
         LaneBytes<D> at;
-        const u32 lds0 = lds_address(&lds[0][0][0]) + wave * 1024;
-        auto request = [&](int t, int buf) {
+        const u32 lds0 = lds_address(&lds[0][0][0][0]) + wave * 1024;
+        auto request = [&](int t, int slot) {
             const int j0 = t * BN, rows = min(BN, n - j0);
             const auto rk = make_rsrc(kp + (int64_t)j0 * a.k_s, (u32)((rows - 1) * a.k_s + D * 2));
             const auto rv = make_rsrc(vp + (int64_t)j0 * a.v_s, (u32)((rows - 1) * a.v_s + D * 2));
@@ -197,68 +200,98 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
             for (int c = 0; c < LPT; ++c) {
                 // behind the sequence's end its last token stands in for the missing ones: no row sees them
                 const int r = my_row + c * (256 / CPR), row = min(r, rows - 1), ch = ((int)threadIdx.x % CPR ^ tile_swizzle<D>(r)) << 4;
-                load_to_lds(rk, lds0 + buf * (2 * kSide) + c * 4096, (int)(row * a.k_s) + ch);
-                load_to_lds(rv, lds0 + buf * (2 * kSide) + kSide + c * 4096, (int)(row * a.v_s) + ch);
+                load_to_lds(rk, lds0 + slot * (2 * kSide) + c * 4096, (int)(row * a.k_s) + ch);
+                load_to_lds(rv, lds0 + slot * (2 * kSide) + kSide + c * 4096, (int)(row * a.v_s) + ch);
             }
         };
-        if (threadIdx.x == 0) odd_tile = -1;
-        int t = walk.next(), buf = 0;
-        bool same = walk.cur_same;
-        int token_doc = 0, doc_next = 0;               // document of token `lane` of the tile, where rows are told apart by it
-        if (t >= 0) {
-            request(t, 0);
-            if constexpr (DOCS)
-                if (!same) doc_next = a.docs[(int64_t)b * a.S + min(t * BN + lane, n - 1)];
-        }
-        while (t >= 0) {
-            const int t_next = walk.next();
-            const bool same_next = walk.cur_same;
+        if (threadIdx.x < PARTS) odd_tile[threadIdx.x] = -1;
+        // the tiles of this round and of the next; t[0] < 0: none are left
+        int t[PARTS], t_next[PARTS], buf = 0;
+        bool same[PARTS], same_next[PARTS];
+        int token_doc = 0, doc_next = 0;               // document of token `lane` of this wave's tile, where rows are told apart by it
+        auto fetch = [&](int into) {
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s) {
+                t_next[s] = s > 0 && t_next[s - 1] < 0 ? -1 : walk.next();
+                same_next[s] = walk.cur_same;
+            }
+            if (into < 0) return;
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s)
+                if (t_next[s] >= 0) {
+                    request(t_next[s], into * PARTS + s);
+                    if constexpr (DOCS)
+                        if (s == part && !same_next[s]) doc_next = a.docs[(int64_t)b * a.S + min(t_next[s] * BN + lane, n - 1)];
+                }
+        };
+        fetch(0);
+        while (t_next[0] >= 0) {
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s) {
+                t[s] = t_next[s];
+                same[s] = same_next[s];
+            }
             wait_tile();
             token_doc = doc_next;
-            if (t_next >= 0) {
-                request(t_next, buf ^ 1);
-                if constexpr (DOCS)
-                    if (!same_next) doc_next = a.docs[(int64_t)b * a.S + min(t_next * BN + lane, n - 1)];
-            }
-            const int j0 = t * BN;
-            uint8_t *kt = lds[buf][0], *vt = lds[buf][1];
+            fetch(buf ^ 1);
+            const int my_t = PARTS == 1 || part == 0 ? t[0] : t[PARTS - 1];
+            const bool my_same = PARTS == 1 || part == 0 ? same[0] : same[PARTS - 1];
+            const int j0 = my_t * BN;
+            uint8_t *kt = lds[buf][part][0], *vt = lds[buf][part][1];
             at.pin();
             // token 32 tb + 8 (r / 4) + r % 4 of the tile is seen if that number is at most lim
             const int lim = min(max(i, prefix - 1), n - 1) - j0 - 4 * half;
-            const bool whole = j0 + BN <= n && same;      // no row misses tokens for their length or document
+            const bool whole = j0 + BN <= n && my_same;      // no row misses tokens for their length or document
             const auto sees = [&](int c) {
                 bool see = c <= lim;
                 if constexpr (DOCS) {
                     const int d0 = __builtin_amdgcn_readlane(token_doc, c), d1 = __builtin_amdgcn_readlane(token_doc, c + 4);
-                    see = see && (same || ((half ? d1 : d0) == my_doc && my_doc >= 0));
+                    see = see && (my_same || ((half ? d1 : d0) == my_doc && my_doc >= 0));
                 }
                 return see;
             };
-            if (!whole || j0 + BN - 1 > max(row0, prefix - 1)) {
-                if (share_nonfinite<D, BN>(vt)) odd_tile = t;
-                lds_barrier();
-                if (odd_tile == t) {
-                    u32 seen = 0;
+            bool edge = false;
 #pragma unroll
-                    for (int c = 0; c < TB * 16; ++c) seen |= sees((c >> 4) * 32 + 8 * ((c & 15) >> 2) + (c & 3)) ? 1u << c : 0u;
-                    note_nonfinite<D, BN>(odd, vt, at, seen);
+            for (int s = 0; s < PARTS; ++s) edge = edge || (t[s] >= 0 && (!same[s] || t[s] * BN + BN > n || t[s] * BN + BN - 1 > max(row0, prefix - 1)));
+            if (edge) {
+                if (my_t >= 0 && share_nonfinite<D, BN, 64 * WAVES>(vt, tid)) odd_tile[part] = my_t;
+                lds_barrier();
+                bool found = odd_tile[0] == t[0];
+                if constexpr (PARTS == 2) found = found || (t[1] >= 0 && odd_tile[1] == t[1]);
+                if (found) {
+                    if (my_t >= 0) {
+                        u32 seen = 0;
+#pragma unroll
+                        for (int c = 0; c < TB * 16; ++c) seen |= sees((c >> 4) * 32 + 8 * ((c & 15) >> 2) + (c & 3)) ? 1u << c : 0u;
+                        note_nonfinite<D, BN>(odd, vt, at, seen);
+                    }
                     lds_barrier();
-                    zero_nonfinite_tile<D, BN>(vt);
+                    if (my_t >= 0) zero_nonfinite_tile<D, BN, 64 * WAVES>(vt, tid);
                     lds_barrier();
                 }
             }
             const int wave_last = min(i0 + 31, n - 1);
-            if (i0 < n && (j0 <= wave_last || j0 < prefix)) {
+            if (my_t >= 0 && i0 < n && (j0 <= wave_last || j0 < prefix)) {
                 f32x16 x[TB];
                 tile_scores<D, BN>(x, kt, at, qf);
-                float factor = modify_block<CAP, TB>(x, a.form);
+                const float factor = modify_block<CAP, TB>(x, a.form);
+                float shift = 0.f;
                 if constexpr (ALIBI) {
-                    const float gap0 = (float)(j0 + 4 * half - i);
+                    const float gap0 = (float)(j0 + 4 * half - i), s = neg_slope / factor;
+                    if (j0 >= prefix || j0 + BN - 1 <= i0) {
+                        // every token that is seen lies before its row: the distance is linear in the token, and the row's part of
+                        // it is the same for the whole tile
+                        shift = -neg_slope * gap0;
 #pragma unroll
-                    for (int tb = 0; tb < TB; ++tb)
+                        for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) x[tb][r] = fmaf(neg_slope, fabsf(gap0 + (float)(tb * 32 + 8 * (r >> 2) + (r & 3))), x[tb][r] * factor);
-                    factor = 1.f;
+                            for (int r = 0; r < 16; ++r) x[tb][r] = fmaf(-s, (float)(tb * 32 + 8 * (r >> 2) + (r & 3)), x[tb][r]);
+                    } else {
+#pragma unroll
+                        for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) x[tb][r] = fmaf(s, fabsf(gap0 + (float)(tb * 32 + 8 * (r >> 2) + (r & 3))), x[tb][r]);
+                    }
                 }
                 if (!whole || j0 + BN - 1 > max(i0, prefix - 1)) {
 #pragma unroll
@@ -267,18 +300,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
                         for (int r = 0; r < 16; ++r) x[tb][r] = sees(tb * 32 + 8 * (r >> 2) + (r & 3)) ? x[tb][r] : kNegInf;
                 }
                 f16x8 p[TB][2];
-                tile_softmax<D, BN>(x, factor, st, o, p);
+                tile_softmax<D, BN>(x, factor, shift, st, o, p);
                 tile_output<D, BN>(o, vt, at, p);
             }
             buf ^= 1;
-            t = t_next;
-            same = same_next;
         }
     }
 
+    float l = halves_sum(st.l);
+    if constexpr (PARTS == 2) {
+        // the second part's sums through LDS, register by register (lane l's words lie next to lane l + 1's), into the first part's
+        lds_barrier();
+        float *box = reinterpret_cast<float *>(&lds[0][0][0][0]) + (wave % WAVES) * (64 * (D / 2 + 2 + D / 32)) + lane;
+        static_assert(WAVES * 64 * (D / 2 + 2 + D / 32) * 4 <= sizeof(lds), "the sums of a part fit into the tiles' memory");
+        if (part == 1) {
+#pragma unroll
+            for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) box[(cb * 16 + r) * 64] = o[cb][r];
+            box[(D / 2) * 64] = st.m;
+            box[(D / 2 + 1) * 64] = l;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int w = 0; w < D / 64; ++w) box[(D / 2 + 2 + s * (D / 64) + w) * 64] = __uint_as_float(odd.hit[s][w]);
+        }
+        lds_barrier();
+        if (part == 1) return;
+        const float m1 = box[(D / 2) * 64], m = fmaxf(st.m, m1);
+        const float f0 = st.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(st.m - m), f1 = m1 == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m1 - m);
+        l = l * f0 + box[(D / 2 + 1) * 64] * f1;       // (zero times an undefined sum is undefined)
+        st.m = m;
+#pragma unroll
+        for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[cb][r] = fmaf(box[(cb * 16 + r) * 64], f1, o[cb][r] * f0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int w = 0; w < D / 64; ++w) odd.hit[s][w] |= __float_as_uint(box[(D / 2 + 2 + s * (D / 64) + w) * 64]);
+    }
     if (i >= a.S) return;
     if (i >= n && !fill) return;
-    const float l = halves_sum(st.l);
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);    // (an undefined sum stays undefined)
     uint8_t *op = out + (((int64_t)b * a.S + i) * a.Hq + hq) * (D * 2);
     if (i >= n) {
@@ -295,7 +358,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void prefill_kernel(PromptAr
             }
     }
     if (lse != nullptr && half == 0)
-        lse[((int64_t)b * a.Hq + hq) * a.S + i] = i < n ? (st.m == kNegInf ? kNegInf : (st.m + __builtin_amdgcn_logf(l)) * kLn2) : kNegInf;
+        lse[((int64_t)b * a.Hq + hq) * a.S + i] = i < n ? (l == 0.f ? kNegInf : (st.m + __builtin_amdgcn_logf(l)) * kLn2) : kNegInf;
 }
 
 // ---- the weight each token received -----------------------------------------------------------------------------------------------
@@ -407,12 +470,20 @@ static int prompt_args(PromptArgs &a, const akv_prompt_desc *d, const char *what
     return AKV_OK;
 }
 
-template <int D, int BN>
+// Two parts a row (64 rows a workgroup) pay only while the workgroups of whole rows leave half of the compute units empty:
+// 512 tokens x 32 heads x 128 14.8 us against 16.6, x 16 heads x 256 24.6 against 33.6; with twice the rows 29.8 against 28.1 (fewer
+// workgroups fit a compute unit, and each tile that is loaded serves half the rows).
+static int prompt_parts(const PromptArgs &a) {
+    AKV_TUNE("AKV_TUNE_PROMPT_PARTS", forced);
+    if (has_forced && (forced == 1 || forced == 2)) return forced;
+    return a.S > 256 && (int64_t)((a.S + 127) / 128) * a.Hq * a.B <= 128 ? 2 : 1;
+}
+template <int D, int BN, int PARTS>
 static void launch_prefill(const PromptArgs &a, bool cap, uint8_t *out, float *lse, int fill, hipStream_t st) {
-    const int n_tiles = (a.S + 127) / 128;
+    const int n_tiles = (a.S + 128 / PARTS - 1) / (128 / PARTS);
     const dim3 grid((u32)((int64_t)n_tiles * a.Hq * a.B));
 #define AKV_PREFILL(CAP, ALIBI, DOCS) \
-    hipLaunchKernelGGL((prefill_kernel<D, BN, CAP, ALIBI, DOCS>), grid, dim3(256), 0, st, a, out, lse, n_tiles, fill)
+    hipLaunchKernelGGL((prefill_kernel<D, BN, PARTS, CAP, ALIBI, DOCS>), grid, dim3(256), 0, st, a, out, lse, n_tiles, fill)
     if (a.docs) {
         if (cap) { if (a.slopes) AKV_PREFILL(true, true, true); else AKV_PREFILL(true, false, true); }
         else { if (a.slopes) AKV_PREFILL(false, true, true); else AKV_PREFILL(false, false, true); }
@@ -438,8 +509,9 @@ extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, 
     if (rc != AKV_OK) return rc;
     AKV_REQUIRE(a.v && out, "prefill_attention: null pointer");
     AKV_REQUIRE(((uintptr_t)out & 15) == 0, "prefill_attention: out must be 16-byte aligned");
-    AKV_REQUIRE((int64_t)((a.S + 127) / 128) * a.Hq * a.B < (1ll << 31), "prefill_attention: too many rows");
+    AKV_REQUIRE((int64_t)((a.S + 63) / 64) * a.Hq * a.B < (1ll << 31), "prefill_attention: too many rows");
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int parts = akv::prompt_parts(a);
     if (a.docs) {
         const size_t need = akv_prefill_attention_workspace_bytes(a.B, a.S);
         AKV_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
@@ -449,12 +521,18 @@ extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, 
         int *order = reinterpret_cast<int *>(ranges + (size_t)a.B * tiles);
         a.doc_tiles = ranges;
         a.order = order;
-        hipLaunchKernelGGL(akv::doc_tiles_kernel, dim3(a.B), dim3(1024), 0, st, a.docs, a.lens, a.prefix, ranges, order, a.S, tiles, tile, (a.S + 127) / 128, 128);
+        hipLaunchKernelGGL(akv::doc_tiles_kernel, dim3(a.B), dim3(1024), 0, st, a.docs, a.lens, a.prefix, ranges, order, a.S, tiles, tile, (a.S + 128 / parts - 1) / (128 / parts), 128 / parts);
     }
     const bool cap = desc->softcap > 0.f;
-    if (desc->head_dim == 64) akv::launch_prefill<64, 64>(a, cap, out, lse, fill_padding, st);
-    else if (desc->head_dim == 128) akv::launch_prefill<128, 64>(a, cap, out, lse, fill_padding, st);
-    else akv::launch_prefill<256, 32>(a, cap, out, lse, fill_padding, st);
+#define AKV_PREFILL_PARTS(D, BN)                                                                                              \
+    do {                                                                                                                     \
+        if (parts == 2) akv::launch_prefill<D, BN, 2>(a, cap, out, lse, fill_padding, st);                                    \
+        else akv::launch_prefill<D, BN, 1>(a, cap, out, lse, fill_padding, st);                                               \
+    } while (0)
+    if (desc->head_dim == 64) AKV_PREFILL_PARTS(64, 64);
+    else if (desc->head_dim == 128) AKV_PREFILL_PARTS(128, 64);
+    else AKV_PREFILL_PARTS(256, 32);
+#undef AKV_PREFILL_PARTS
     return akv::check_launch("prefill_attention");
 }
 

@@ -259,3 +259,26 @@ def test_accumulate_weights(ops, B, Hq, Hkv, cap, width, decay):
         assert ((w[b, :, :n].double() - want).abs() <= (Hq // Hkv + 1) * U32 * want).all()
         assert torch.equal(other[b, :, :n], w[b, :, :n])
         assert torch.equal(w[b, :, n:], before[b, :, n:]) and (other[b, :, n:] == 5).all()
+
+
+@pytest.mark.parametrize("parts", ["1", "2"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_whole_rows_and_rows_in_two_parts(ops, monkeypatch, parts, D):
+    """Both forms of the kernel on the same calls: a workgroup's rows as one run over the tokens, or split over two halves of its waves."""
+    from alignedkv_amd import load_library
+    lib = load_library()
+    monkeypatch.setenv("AKV_TUNE_PROMPT_PARTS", parts)
+    lib.akv_reload_tuning()
+    try:
+        i32 = dict(dtype=torch.int32, device="cuda")
+        for S in (1, 33, 64, 65, 130, 300, 389):
+            q, k, v = inputs(2, S, 4, 2, D, seed=S)
+            lens, prefix = torch.tensor([S, S // 2], **i32), torch.tensor([S // 3, 100], **i32)
+            docs = torch.sort(torch.randint(-1, 4, (2, S)), 1).values.to(torch.int32).cuda()
+            for kw in (dict(), dict(seq_lens=lens, prefix_lens=prefix, softcap=5.0), dict(documents=docs, seq_lens=lens, slopes=slopes_of(4))):
+                out, lse = ops.prefill_attention(q, k, v, return_lse=True, **kw)
+                check_against_form(out, lse, q, k, v, kw.get("softcap", 0.0), kw.get("slopes"), kw.get("seq_lens"), kw.get("prefix_lens"), kw.get("documents"))
+        test_values_that_are_not_numbers_reach_the_rows_that_see_them_and_no_others(ops)
+    finally:
+        monkeypatch.delenv("AKV_TUNE_PROMPT_PARTS")
+        lib.akv_reload_tuning()
