@@ -222,13 +222,6 @@ __device__ __forceinline__ bool share_nonfinite(const uint8_t *v_tile, int tid) 
     }
     return __any(most.x >= 0x7C00 || most.y >= 0x7C00);
 }
-__device__ __forceinline__ bool any_nonfinite(f16x8 v) {
-    const u32x4 w = __builtin_bit_cast(u32x4, v);
-    u32 hit = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) hit |= ((w[i] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;    // (an exponent of all ones carries out)
-    return hit != 0;
-}
 __device__ __forceinline__ f16x8 zero_nonfinite(f16x8 v) {
     u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll

@@ -19,376 +19,309 @@ struct TreeArgs {
     uint8_t *out;
     float *parts;                         // [B * Hkv, splits, rows] x {D sums}, then the same x {m, l}
     int T, Hq, G, rows;                   // rows = T * G
-    int plane_splits, tiles_per_split, splits;
+    int plane_splits, tokens_per_split, splits;
     ScoreForm form;
 };
 
 // Cached tokens of a sequence, kept inside the planes whatever the device holds.
 __device__ __forceinline__ int cached_tokens(const TreeArgs &a, int b) { return max(0, min(a.c.seq_lens[b], a.c.max_seq_len)); }
 
-// acc[t] += K (tokens) x Q^T for one step of 32 channels.  A lane (m, kg) holds 8 channels x TPL tokens of token set m; operand t
-// is token t of every set, so no value leaves its lane.
-template <int TPL>
-struct KStep {
-    u32 h[8][TPL / 4], m[8][TPL / 8], l[8][TPL / 8];
-};
-
-template <int N>
-__device__ __forceinline__ void load_words(u32 (&w)[N], __amdgpu_buffer_rsrc_t r, int off) {
-    if constexpr (N == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kStream);
-    if constexpr (N == 2) {
-        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kStream);
-        w[0] = x.x;
-        w[1] = x.y;
-    }
-    if constexpr (N == 4) {
-        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, kStream);
-        w[0] = x.x;
-        w[1] = x.y;
-        w[2] = x.z;
-        w[3] = x.w;
-    }
-}
-
-// 16-bit values of elements 0,2 / 1,3 / 4,6 / 5,7 of 8 elements (high bytes Ha, Hb; nibbles M, L)
-__device__ __forceinline__ void rebuild8(u32 Ha, u32 Hb, u32 M, u32 L, u32 &w02, u32 &w13, u32 &w46, u32 &w57) {
+// 16-bit values of elements 0,2 / 1,3 / 4,6 / 5,7 of 8 elements (high bytes Ha, Hb; nibbles M, L).  They are used in this order: four
+// elements 0 1 2 3 lie at places 0 2 1 3, which costs nothing where the order of tokens or channels is free.
+__device__ __forceinline__ u32x4 rebuild8(u32 Ha, u32 Hb, u32 M, u32 L) {
     u32 E, O;
     split_even_odd(M, L, E, O);
-    w02 = __builtin_amdgcn_perm(Ha, E, 0x06010400u);
-    w13 = __builtin_amdgcn_perm(Ha, O, 0x07010500u);
-    w46 = __builtin_amdgcn_perm(Hb, E, 0x06030402u);
-    w57 = __builtin_amdgcn_perm(Hb, O, 0x07030502u);
+    return u32x4{__builtin_amdgcn_perm(Ha, E, 0x06010400u), __builtin_amdgcn_perm(Ha, O, 0x07010500u), __builtin_amdgcn_perm(Hb, E, 0x06030402u),
+                 __builtin_amdgcn_perm(Hb, O, 0x07030502u)};
 }
-__device__ __forceinline__ u32 low_halves(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
-__device__ __forceinline__ u32 high_halves(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-
-// 8 x 8 block of halves held as w[i] (i: index of the pair partner list) -> operand dwords.  in: for each of 8 rows i the words
-// {02, 13, 46, 57} of 8 columns; out[c][p]: column c, rows 2 p and 2 p + 1.
-__device__ __forceinline__ void transpose8(const u32 (&w)[8][4], u32 (&out)[8][4]) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        const u32 (&a)[4] = w[2 * p], (&b)[4] = w[2 * p + 1];
-        out[0][p] = low_halves(a[0], b[0]);
-        out[2][p] = high_halves(a[0], b[0]);
-        out[1][p] = low_halves(a[1], b[1]);
-        out[3][p] = high_halves(a[1], b[1]);
-        out[4][p] = low_halves(a[2], b[2]);
-        out[6][p] = high_halves(a[2], b[2]);
-        out[5][p] = low_halves(a[3], b[3]);
-        out[7][p] = high_halves(a[3], b[3]);
-    }
-}
-__device__ __forceinline__ f16x8 operand(const u32 (&w)[4]) { return as_f16x8(u32x4{w[0], w[1], w[2], w[3]}); }
-
-// Over the four lanes n, n + 16, n + 32, n + 48 of a column.
-__device__ __forceinline__ float column_max(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float column_sum(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+__host__ __device__ constexpr int place(int x) { return (x & ~3) | (x & 1) << 1 | (x >> 1 & 1); }    // (its own inverse)
+// eight fp16 values in memory order, brought into that order
+__device__ __forceinline__ u32x4 placed(u32x4 w) {
+    return u32x4{__builtin_amdgcn_perm(w.y, w.x, 0x05040100u), __builtin_amdgcn_perm(w.y, w.x, 0x07060302u), __builtin_amdgcn_perm(w.w, w.z, 0x05040100u),
+                 __builtin_amdgcn_perm(w.w, w.z, 0x07060302u)};
 }
 
-// One wave's running state for NT x 16 query rows: a lane owns column n = lane & 15 of every tile of rows.
-template <int D, int NT>
-struct Rows {
-    static constexpr int CPL = D / 16;        // channels of a lane's set: channel CPL * (4 kg + r) + j
-    f16x8 q[NT][D / 32];
-    f32x4 o[NT][CPL];
-    float m[NT], l[NT];
-    unsigned long long anc[NT];
-    int pos[NT];                              // the row's position
-    float neg_slope[NT];
+// 16 elements of a plane triple: one channel of 16 tokens (keys) or 16 channels of one token (values).
+struct Raw16 {
+    u32x4 h;
+    u32x2 m, l;
 };
-
-// x[i] (units of log2 e, -inf where hidden), N values of one column per lane -> probabilities, state and outputs rescaled.
-template <int D, int NT, int N>
-__device__ __forceinline__ void rows_softmax(float (&x)[N], Rows<D, NT> &s, int nt) {
-    float mx = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-    mx = column_max(mx);
-    if (__any(mx > s.m[nt] + 8.f)) {
-        const float m_new = fmaxf(s.m[nt], mx);
-        const float alpha = s.m[nt] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(s.m[nt] - m_new);
-        s.m[nt] = m_new;
-        s.l[nt] *= alpha;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) s.o[nt][j] *= alpha;
-    }
-    const float m = s.m[nt] == kNegInf ? 0.f : s.m[nt];
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        x[i] = __builtin_amdgcn_exp2f(x[i] - m);
-        sum += x[i];
-    }
-    s.l[nt] += sum;
+__device__ __forceinline__ Raw16 load_raw16(__amdgpu_buffer_rsrc_t rh, __amdgpu_buffer_rsrc_t rm, __amdgpu_buffer_rsrc_t rl, int off, bool in) {
+    Raw16 r;
+    r.h = __builtin_amdgcn_raw_buffer_load_b128(rh, in ? off : kSkip, 0, 0);
+    r.m = __builtin_amdgcn_raw_buffer_load_b64(rm, in ? off >> 1 : kSkip, 0, 0);
+    r.l = __builtin_amdgcn_raw_buffer_load_b64(rl, in ? off >> 1 : kSkip, 0, 0);
+    return r;
 }
 
-// One tile of 16 * TPL tokens of the planes starting at token j0 (a multiple of 64), n_valid of them in the planes (a multiple of 64).
-template <int D, int KB, int TPL, int NT, bool CAP, bool ALIBI>
-__device__ __forceinline__ void plane_tile(const TreeArgs &a, Rows<D, NT> &s, int64_t bh, int j0, int n_valid) {
-    constexpr int CPL = D / 16;
-    const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4;
-    const bool k_in = m * TPL < n_valid, v_in = kg * 4 * TPL < n_valid;
-    f32x4 acc[NT][TPL];
+// Keys in LDS: [channel][BN tokens] fp16, as the planes have them.  The operand of a score product wants eight channels of one
+// token a lane: two transposing reads of four channels each.
+template <int BN>
+__device__ __forceinline__ int key_byte(int channel, int chunk) {
+    if constexpr (BN == 64) return tile_byte<64>(channel, chunk);
+    return channel * 64 + chunk * 16;      // (a read takes whole rows here: they do not collide)
+}
+template <int D, int BN>
+__device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t *k_tile, int at0, int at1, const f16x8 (&qf)[D / 16]) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int tb = 0; tb < BN / 32; ++tb)
 #pragma unroll
-        for (int t = 0; t < TPL; ++t) acc[nt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    {
+        for (int r = 0; r < 16; ++r) acc[tb][r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+        for (int tb = 0; tb < BN / 32; ++tb) {
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(k_tile + (at0 ^ (tb << 6)) + ks * 16 * BN * 2));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(k_tile + (at1 ^ (tb << 6)) + ks * 16 * BN * 2));
+            acc[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)), qf[ks], acc[tb], 0, 0, 0);
+        }
+        if (ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// grid (splits, Hkv * row groups, B), 256 threads.  Split s < plane_splits: tiles of the planes; the last split: the rest buffer and the
+// drafts.  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
+// unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
+// 128 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
+// tree_combine_kernel.
+template <int D, int KB, int PARTS, int BN, bool CAP, bool ALIBI>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
+    constexpr int TT = PARTS * BN, ROWS = 128 / PARTS, WAVES = 4 / PARTS, TB = BN / 32;
+    constexpr int UNITS = D * TT / 16 / 256;         // Raw16 of each side per thread and round
+    constexpr int kPart = D * BN * 2;
+    constexpr int kBox = 64 * (D / 2 + 2 + D / 32);  // words a wave hands over when the parts are joined
+    constexpr int kLds = 2 * PARTS * kPart > (PARTS - 1) * WAVES * kBox * 4 ? 2 * PARTS * kPart : (PARTS - 1) * WAVES * kBox * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+    __shared__ int tail_pos[128];                    // positions of the tail's tokens
+    __shared__ int odd_tile[PARTS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), half = lane >> 5, part = wave / WAVES, part_tid = tid & (64 * WAVES - 1);
+    const int groups = (a.rows + ROWS - 1) / ROWS;
+    const int split = blockIdx.x, hkv = blockIdx.y / groups, rg = blockIdx.y - hkv * groups, b = blockIdx.z;
+    const int n = cached_tokens(a, b), flushed = n / kRest * kRest, n_rest = n - flushed, total = n_rest + a.T;
+    const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv;
+    const int row = rg * ROWS + (wave % WAVES) * 32 + (lane & 31), row_c = min(row, a.rows - 1), g = row_c / a.T, t = row_c - g * a.T;
+    const bool tail = split == a.plane_splits;
+    uint8_t *kt = lds + part * kPart, *vt = lds + PARTS * kPart + part * kPart;
+
+    // the planes: this thread's pieces of a round
+    const int first = split * a.tokens_per_split, end = tail ? 0 : min(first + a.tokens_per_split, flushed);
+    Raw16 kr[UNITS], vr[UNITS];
+    auto request_k = [&](int j0) {
         const int64_t blk = bh * a.c.n_max_blocks + j0 / KB;
-        const int blocks = KB == 64 ? (n_valid + 63) / 64 : 1, tok0 = j0 % KB + m * TPL;
+        const int blocks = min(KB == 64 ? TT / 64 + (TT < 64) : 1, a.c.n_max_blocks - j0 / KB);
         const auto rh = make_rsrc(a.c.k_first_8 + blk * (D * KB), blocks * D * KB);
         const auto rm = make_rsrc(a.c.k_mid_4 + blk * (D * KB / 2), blocks * D * KB / 2);
         const auto rl = make_rsrc(a.c.k_last_4 + blk * (D * KB / 2), blocks * D * KB / 2);
-        const int base = KB == 64 ? (tok0 / 64) * (D * 64) + tok0 % 64 : tok0;
 #pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks) {
-            KStep<TPL> w;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int off = base + (ks * 32 + kg * 8 + i) * KB;
-                load_words(w.h[i], rh, k_in ? off : kSkip);
-                load_words(w.m[i], rm, k_in ? off >> 1 : kSkip);
-                load_words(w.l[i], rl, k_in ? off >> 1 : kSkip);
-            }
-#pragma unroll
-            for (int g = 0; g < TPL / 8; ++g) {
-                u32 in[8][4], op[8][4];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) rebuild8(w.h[i][2 * g], w.h[i][2 * g + 1], w.m[i][g], w.l[i][g], in[i][0], in[i][1], in[i][2], in[i][3]);
-                transpose8(in, op);
-#pragma unroll
-                for (int t = 0; t < 8; ++t)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        acc[nt][8 * g + t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(op[t]), s.q[nt][ks], acc[nt][8 * g + t], 0, 0, 0);
-            }
+        for (int u = 0; u < UNITS; ++u) {
+            const int id = u * 256 + tid, tok = id % (TT / 16) * 16, ch = id / (TT / 16), in = j0 % KB + tok;
+            kr[u] = load_raw16(rh, rm, rl, in / KB * (D * KB) + ch * KB + in % KB, j0 + tok < end);
         }
-    }
-    // lane (n, kg): token TPL * (4 kg + r) + t of the tile in acc[t][r]
-    u32 p[NT][TPL * 4 / 8][4];
+    };
+    auto request_v = [&](int j0) {
+        const int64_t r0 = bh * a.c.max_seq_len + j0;
+        const int rows = end - j0;
+        const auto rh = make_rsrc(a.c.v_first_8 + r0 * D, min(rows, TT) * D);
+        const auto rm = make_rsrc(a.c.v_mid_4 + r0 * (D / 2), min(rows, TT) * D / 2);
+        const auto rl = make_rsrc(a.c.v_last_4 + r0 * (D / 2), min(rows, TT) * D / 2);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float x[4 * TPL];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int t = 0; t < TPL; ++t) {
-                float y = modified<CAP>(acc[nt][t][r], a.form);
-                if constexpr (ALIBI) y = fmaf(s.neg_slope[nt], fabsf((float)(s.pos[nt] - (j0 + TPL * (4 * kg + r) + t))), y);
-                x[r * TPL + t] = v_in ? y : kNegInf;
-            }
-        rows_softmax<D, NT, 4 * TPL>(x, s, nt);
-#pragma unroll
-        for (int st = 0; st < TPL / 2; ++st)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[nt][st][i] = pack_f16(x[8 * st + 2 * i], x[8 * st + 2 * i + 1]);
-    }
-    {
-        // eight consecutive tokens per step and lane, channels CPL * m .. of each
-        const int64_t row0 = bh * a.c.max_seq_len + j0;
-        const auto rh = make_rsrc(a.c.v_first_8 + row0 * D, n_valid * D);
-        const auto rm = make_rsrc(a.c.v_mid_4 + row0 * (D / 2), n_valid * D / 2);
-        const auto rl = make_rsrc(a.c.v_last_4 + row0 * (D / 2), n_valid * D / 2);
-#pragma unroll
-        for (int st = 0; st < TPL / 2; ++st) {
-            u32 h[8][(CPL + 3) / 4], md[8][(CPL + 7) / 8], ls[8][(CPL + 7) / 8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int off = (kg * 4 * TPL + 8 * st + i) * D + CPL * m;
-                load_words(h[i], rh, v_in ? off : kSkip);
-                if constexpr (CPL == 4) {
-                    md[i][0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rm, v_in ? off >> 1 : kSkip, 0, kStream);
-                    ls[i][0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rl, v_in ? off >> 1 : kSkip, 0, kStream);
-                } else {
-                    load_words(md[i], rm, v_in ? off >> 1 : kSkip);
-                    load_words(ls[i], rl, v_in ? off >> 1 : kSkip);
-                }
-            }
-#pragma unroll
-            for (int g = 0; g < (CPL + 7) / 8; ++g) {
-                u32 in[8][4], op[8][4];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    rebuild8(h[i][2 * g], CPL == 4 ? 0u : h[i][(2 * g + 1) % ((CPL + 3) / 4)], md[i][g], ls[i][g], in[i][0], in[i][1], in[i][2], in[i][3]);
-                transpose8(in, op);
-#pragma unroll
-                for (int c = 0; c < (CPL < 8 ? CPL : 8); ++c)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        s.o[nt][8 * g + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(op[c]), operand(p[nt][st]), s.o[nt][8 * g + c], 0, 0, 0);
-            }
+        for (int u = 0; u < UNITS; ++u) {
+            const int id = u * 256 + tid, c16 = id % (D / 16), tok = id / (D / 16);
+            vr[u] = load_raw16(rh, rm, rl, tok * D + c16 * 16, tok < rows);
         }
+    };
+    auto put_k = [&]() {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int id = u * 256 + tid, tok = id % (TT / 16) * 16, ch = id / (TT / 16);
+            uint8_t *to = lds + tok / BN * kPart;
+            *reinterpret_cast<u32x4 *>(to + key_byte<BN>(ch, tok % BN / 8)) = rebuild8(kr[u].h.x, kr[u].h.y, kr[u].m.x, kr[u].l.x);
+            *reinterpret_cast<u32x4 *>(to + key_byte<BN>(ch, tok % BN / 8 + 1)) = rebuild8(kr[u].h.z, kr[u].h.w, kr[u].m.y, kr[u].l.y);
+        }
+    };
+    auto put_v = [&]() {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            const int id = u * 256 + tid, c16 = id % (D / 16), tok = id / (D / 16);
+            uint8_t *to = lds + PARTS * kPart + tok / BN * kPart;
+            *reinterpret_cast<u32x4 *>(to + tile_byte<D>(place(tok % BN), 2 * c16)) = rebuild8(vr[u].h.x, vr[u].h.y, vr[u].m.x, vr[u].l.x);
+            *reinterpret_cast<u32x4 *>(to + tile_byte<D>(place(tok % BN), 2 * c16 + 1)) = rebuild8(vr[u].h.z, vr[u].h.w, vr[u].m.y, vr[u].l.y);
+        }
+    };
+    // (V of a round is asked for behind its K: both at once do not fit beside the sums, except where a wave has a SIMD to itself)
+    constexpr bool kAhead = D == 64;
+    if (first < end) {
+        request_k(first);
+        if constexpr (kAhead) request_v(first);
     }
-}
 
-// 32 tokens of the tail: the rest buffer's n_rest tokens, then the T drafts; u0: first token of this tile.
-template <int D, int NT, bool CAP, bool ALIBI>
-__device__ __forceinline__ void tail_tile(const TreeArgs &a, Rows<D, NT> &s, int b, int hkv, int u0, int n_rest, int n) {
-    constexpr int CPL = D / 16;
-    const int lane = threadIdx.x & 63, m = lane & 15, kg = lane >> 4, H = a.c.n_kv_heads, total = n_rest + a.T;
-    const uint8_t *rk = a.c.restk + ((int64_t)b * kRest * H + hkv) * (D * 2), *rv = a.c.restv + ((int64_t)b * kRest * H + hkv) * (D * 2);
-    const uint8_t *dk = a.k + ((int64_t)b * a.T * H + hkv) * (D * 2), *dv = a.v + ((int64_t)b * a.T * H + hkv) * (D * 2);
-    const int64_t row_bytes = (int64_t)H * D * 2;
-    const auto k_row = [&](int u) { return u < n_rest ? rk + u * row_bytes : dk + (min(u, total - 1) - n_rest) * row_bytes; };
-    const auto v_row = [&](int u) { return u < n_rest ? rv + u * row_bytes : dv + (min(u, total - 1) - n_rest) * row_bytes; };
-    f32x4 acc[NT][2];
+    f16x8 qf[D / 16];
+    const uint8_t *qp = a.q + (((int64_t)b * a.T + t) * a.Hq + hkv * a.G + g) * (D * 2);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const uint8_t *kp = k_row(u0 + 16 * t + m);
-#pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks) {
-            const f16x8 w = *reinterpret_cast<const f16x8 *>(kp + (ks * 32 + kg * 8) * 2);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, s.q[nt][ks], acc[nt][t], 0, 0, 0);
-        }
-    }
-    // lane (n, kg): token u0 + 16 t + 4 kg + r in acc[t][r]
+    for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const f16x8 *>(qp + (2 * ks + half) * 16);
     const unsigned long long *anc = a.anc + (int64_t)b * a.anc_stride;
-    const auto visible = [&](int nt, int u) { return u < n_rest || (u < total && ((s.anc[nt] >> (u - n_rest)) & 1)); };
-    u32 p[NT][4];
+    const unsigned long long my_anc = anc[t];
+    const int pos = n + __popcll(my_anc & ~(1ull << t));
+    const float neg_slope = ALIBI ? a.slopes[hkv * a.G + g] * -kLog2e : 0.f;
+    LaneBytes<D> at;
+    const int kr0 = 8 * half + ((lane & 15) >> 2), kchunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    int k_at0 = key_byte<BN>(kr0, kchunk) + (lane & 1) * 8, k_at1 = key_byte<BN>(kr0 + 4, kchunk) + (lane & 1) * 8;
+    f32x16 o[D / 32];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        float x[8];
+    for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int u = u0 + 16 * t + 4 * kg + r;
-                float y = modified<CAP>(acc[nt][t][r], a.form);
-                if constexpr (ALIBI) {
-                    const int d = min(max(u - n_rest, 0), a.T - 1);
-                    const int at = u < n_rest ? n - n_rest + u : n + __popcll(anc[d] & ~(1ull << d));
-                    y = fmaf(s.neg_slope[nt], fabsf((float)(s.pos[nt] - at)), y);
-                }
-                x[4 * t + r] = visible(nt, u) ? y : kNegInf;
-            }
-        rows_softmax<D, NT, 8>(x, s, nt);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[nt][i] = pack_f16(x[2 * i], x[2 * i + 1]);
-    }
-    bool bad = false;
-#pragma unroll
-    for (int g = 0; g < (CPL + 7) / 8; ++g) {
-        u32 in[8][4], op[8][4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int u = u0 + 16 * (i >> 2) + 4 * kg + (i & 3);
-            const uint8_t *vp = v_row(u) + (CPL * m + 8 * g) * 2;
-            const u32 w0 = *reinterpret_cast<const u32 *>(vp), w1 = *reinterpret_cast<const u32 *>(vp + 4);
-            u32 w2 = 0, w3 = 0;
-            if constexpr (CPL >= 8) {
-                w2 = *reinterpret_cast<const u32 *>(vp + 8);
-                w3 = *reinterpret_cast<const u32 *>(vp + 12);
-            }
-            in[i][0] = low_halves(w0, w1);
-            in[i][1] = high_halves(w0, w1);
-            in[i][2] = low_halves(w2, w3);
-            in[i][3] = high_halves(w2, w3);
-        }
-        transpose8(in, op);
-#pragma unroll
-        for (int c = 0; c < (CPL < 8 ? CPL : 8); ++c) {
-            bad |= any_nonfinite(operand(op[c]));
-            const f16x8 w = zero_nonfinite(operand(op[c]));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                s.o[nt][8 * g + c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, operand(p[nt]), s.o[nt][8 * g + c], 0, 0, 0);
-        }
-    }
-    if (!__any(bad)) return;
-    // infinite or undefined values reach exactly the rows that see their token
-#pragma unroll 1
-    for (int u = u0; u < min(u0 + 32, total); ++u) {
-        const uint8_t *vp = v_row(u);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (!visible(nt, u)) continue;
-#pragma unroll
-            for (int j = 0; j < CPL; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float f = (float)*reinterpret_cast<const _Float16 *>(vp + (CPL * (4 * kg + r) + j) * 2);
-                    if (!(fabsf(f) < __builtin_inff())) s.o[nt][j][r] += f;
-                }
-        }
-    }
-}
+        for (int r = 0; r < 16; ++r) o[cb][r] = 0.f;
+    RowState st;
+    OddValues<D> odd;
 
-// grid (splits, Hkv * row groups, B), 256 threads.  Split s < plane_splits: tiles of the planes, one a wave at a time; the last split: the
-// rest buffer and the drafts.  The four waves of a workgroup join their rows' sums through LDS and write one partial result.
-template <int D, int KB, int TPL, int NT, bool CAP, bool ALIBI>
-__global__ __launch_bounds__(256) void tree_kernel(TreeArgs a) {
-    constexpr int CPL = D / 16, TOK = 16 * TPL;
-    __shared__ float part[4][16][D + 4];
-    __shared__ float ms[4][16], ls[4][16];
-    const int lane = threadIdx.x & 63, wave = wave_index(), n_col = lane & 15, kg = lane >> 4;
-    const int groups = (a.rows + NT * 16 - 1) / (NT * 16);
-    const int split = blockIdx.x, hkv = blockIdx.y / groups, rg = blockIdx.y - hkv * groups, b = blockIdx.z;
-    const int n = cached_tokens(a, b), flushed = n / kRest * kRest, n_rest = n - flushed;
-    const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv;
-    Rows<D, NT> s;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int row = min(rg * NT * 16 + nt * 16 + n_col, a.rows - 1), g = row / a.T, t = row - g * a.T;
-        const uint8_t *qp = a.q + (((int64_t)b * a.T + t) * a.Hq + hkv * a.G + g) * (D * 2);
-#pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks) s.q[nt][ks] = *reinterpret_cast<const f16x8 *>(qp + (ks * 32 + kg * 8) * 2);
-#pragma unroll
-        for (int j = 0; j < CPL; ++j) s.o[nt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        s.m[nt] = kNegInf;
-        s.l[nt] = 0.f;
-        s.anc[nt] = a.anc[(int64_t)b * a.anc_stride + t];
-        s.pos[nt] = n + __popcll(s.anc[nt] & ~(1ull << t));
-        s.neg_slope[nt] = ALIBI ? a.slopes[hkv * a.G + g] * -kLog2e : 0.f;
-    }
-    if (split < a.plane_splits) {
-        const int first = split * a.tiles_per_split, end = min(first + a.tiles_per_split, (flushed + TOK - 1) / TOK);
-        for (int t = first + wave; t < end; t += 4)
-            plane_tile<D, KB, TPL, NT, CAP, ALIBI>(a, s, bh, t * TOK, min(TOK, flushed - t * TOK));
-    } else {
-        for (int u0 = wave * 32; u0 < n_rest + a.T; u0 += 128) tail_tile<D, NT, CAP, ALIBI>(a, s, b, hkv, u0, n_rest, n);
-    }
-    float *po = a.parts + (bh * a.splits + split) * (int64_t)a.rows * D;
-    float *pm = a.parts + (int64_t)a.c.bsz * a.c.n_kv_heads * a.splits * a.rows * D + (bh * a.splits + split) * (int64_t)a.rows * 2;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const float l = column_sum(s.l[nt]);
-        if (kg == 0) {
-            ms[wave][n_col] = s.m[nt];
-            ls[wave][n_col] = l;
+    for (int j0 = first; j0 < end; j0 += TT) {
+        at.pin();
+        asm volatile("" : "+v"(k_at0), "+v"(k_at1));
+        put_k();
+        const int next = j0 + TT;
+        if constexpr (kAhead) {
+            if (next < end) request_k(next);
+        } else {
+            request_v(j0);
         }
+        lds_barrier();
+        const int jp = j0 + part * BN;              // this wave's tokens: whole 64s or none (32: the valid ones come first)
+        const bool mine = jp < end;
+        f32x16 x[TB];
+        f16x8 p[TB][2];
+        float factor = 1.f, shift = 0.f;
+        if (mine) {
+            key_scores<D, BN>(x, kt, k_at0, k_at1, qf);
+            factor = modify_block<CAP, TB>(x, a.form);
+            if constexpr (ALIBI) {
+                // every cached token lies before the row: the distance is linear in the token
+                const float s = neg_slope / factor;
+                shift = -neg_slope * (float)(jp + 4 * half - pos);
 #pragma unroll
-        for (int j = 0; j < CPL; ++j)
+                for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) part[wave][n_col][CPL * (4 * kg + r) + j] = s.o[nt][j][r];
-        __syncthreads();
-        for (int id = threadIdx.x; id < 16 * D; id += 256) {
-            const int col = id / D, ch = id - col * D, row = rg * NT * 16 + nt * 16 + col;
-            const float m = fmaxf(fmaxf(ms[0][col], ms[1][col]), fmaxf(ms[2][col], ms[3][col]));
-            float o = 0.f, sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = ms[w][col] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms[w][col] - m);
-                // a wave that saw nothing has sums of zero, unless a value it did see was undefined: then so is the row
-                o += part[w][col][ch] * f;
-                sum += ls[w][col] * f;
+                    for (int r = 0; r < 16; ++r) x[tb][r] = fmaf(-s, (float)(tb * 32 + 8 * (r >> 2) + place(r & 3)), x[tb][r]);
             }
-            if (row < a.rows) {
-                po[(int64_t)row * D + ch] = o;
-                if (ch == 0) {
-                    pm[row * 2] = m;
-                    pm[row * 2 + 1] = sum;
+            tile_softmax<D, BN>(x, factor, shift, st, o, p);
+        }
+        put_v();
+        if (next < end) {
+            if constexpr (kAhead) request_v(next);
+            else request_k(next);
+        }
+        lds_barrier();
+        if (mine) tile_output<D, BN>(o, vt, at, p);
+    }
+
+    if (tail) {
+        // the rest buffer and the drafts: fp16 rows, keys and values token-major in LDS
+        const int H = a.c.n_kv_heads;
+        const int64_t row_bytes = (int64_t)H * D * 2, r0 = ((int64_t)b * kRest * H + hkv) * (D * 2), d0 = ((int64_t)b * a.T * H + hkv) * (D * 2);
+        if (tid < total) tail_pos[tid] = tid < n_rest ? flushed + tid : n + __popcll(anc[tid - n_rest] & ~(1ull << (tid - n_rest)));
+        if (tid < PARTS) odd_tile[tid] = -1;
+        constexpr int CPR = D / 8;
+        for (int u0 = 0; u0 < total; u0 += TT) {
+            lds_barrier();
+#pragma unroll 2
+            for (int id = tid; id < TT * CPR; id += 256) {
+                const int u = id / CPR, ch = id % CPR, uu = u0 + u;
+                u32x4 kw = {0u, 0u, 0u, 0u}, vw = {0u, 0u, 0u, 0u};
+                if (uu < total) {
+                    const bool old = uu < n_rest;
+                    const int64_t off = (old ? r0 + uu * row_bytes : d0 + (uu - n_rest) * row_bytes) + ch * 16;
+                    kw = *reinterpret_cast<const u32x4 *>((old ? a.c.restk : a.k) + off);
+                    vw = *reinterpret_cast<const u32x4 *>((old ? a.c.restv : a.v) + off);
                 }
+                *reinterpret_cast<u32x4 *>(lds + u / BN * kPart + tile_byte<D>(u % BN, ch)) = kw;
+                *reinterpret_cast<u32x4 *>(lds + PARTS * kPart + u / BN * kPart + tile_byte<D>(u % BN, ch)) = placed(vw);
+            }
+            lds_barrier();
+            const int up = u0 + part * BN;
+            const auto token = [&](int c) { return up + 4 * half + (c >> 4) * 32 + 8 * ((c & 15) >> 2) + (c & 3); };   // of register c % 16 of block c / 16
+            u32 seen = 0;
+#pragma unroll
+            for (int c = 0; c < TB * 16; ++c) {
+                const int u = token(c);
+                seen |= u < n_rest || (u < total && ((my_anc >> ((u - n_rest) & 63)) & 1)) ? 1u << c : 0u;
+            }
+            if (up < total && share_nonfinite<D, BN, 64 * WAVES>(vt, part_tid)) odd_tile[part] = u0;
+            lds_barrier();
+            bool found = false;
+#pragma unroll
+            for (int s = 0; s < PARTS; ++s) found = found || odd_tile[s] == u0;
+            if (found) {
+                note_nonfinite<D, BN>(odd, vt, at, seen);
+                lds_barrier();
+                zero_nonfinite_tile<D, BN, 64 * WAVES>(vt, part_tid);
+                lds_barrier();
+            }
+            if (up < total) {
+                f32x16 x[TB];
+                f16x8 p[TB][2];
+                tile_scores<D, BN>(x, kt, at, qf);
+                const float factor = modify_block<CAP, TB>(x, a.form);
+                const float s = ALIBI ? neg_slope / factor : 0.f;
+#pragma unroll
+                for (int c = 0; c < TB * 16; ++c) {
+                    float y = x[c >> 4][c & 15];
+                    if constexpr (ALIBI) y = fmaf(s, fabsf((float)(pos - tail_pos[min(token(c), total - 1)])), y);
+                    x[c >> 4][c & 15] = (seen >> c) & 1 ? y : kNegInf;
+                    if (c % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+                }
+                tile_softmax<D, BN>(x, factor, 0.f, st, o, p);
+                tile_output<D, BN>(o, vt, at, p);
             }
         }
-        if (nt + 1 < NT) __syncthreads();
+    }
+
+    float l = halves_sum(st.l);
+    if (odd.any()) odd.add(o);
+    if constexpr (PARTS > 1) {
+        lds_barrier();
+        float *box = reinterpret_cast<float *>(lds) + lane;
+        if (part > 0) {
+            float *to = box + ((part - 1) * WAVES + wave % WAVES) * kBox;
+#pragma unroll
+            for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[(cb * 16 + r) * 64] = o[cb][r];
+            to[(D / 2) * 64] = st.m;
+            to[(D / 2 + 1) * 64] = l;
+        }
+        lds_barrier();
+        if (part > 0) return;
+        float m = st.m;
+#pragma unroll
+        for (int s = 1; s < PARTS; ++s) m = fmaxf(m, box[((s - 1) * WAVES + wave) * kBox + (D / 2) * 64]);
+        const float f0 = st.m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+        l *= f0;
+#pragma unroll
+        for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[cb][r] *= f0;
+#pragma unroll
+        for (int s = 1; s < PARTS; ++s) {
+            const float *from = box + ((s - 1) * WAVES + wave) * kBox;
+            const float ms = from[(D / 2) * 64], f = ms == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+            l = fmaf(from[(D / 2 + 1) * 64], f, l);
+#pragma unroll
+            for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[cb][r] = fmaf(from[(cb * 16 + r) * 64], f, o[cb][r]);
+        }
+        st.m = m;
+    }
+    if (row >= a.rows) return;
+    float *po = a.parts + ((bh * a.splits + split) * a.rows + row) * D;
+    float *pm = a.parts + (int64_t)a.c.bsz * a.c.n_kv_heads * a.splits * a.rows * D + ((bh * a.splits + split) * a.rows + row) * 2;
+#pragma unroll
+    for (int cb = 0; cb < D / 32; ++cb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4 *>(po + cb * 32 + 8 * q + 4 * half) = f32x4{o[cb][4 * q], o[cb][4 * q + 2], o[cb][4 * q + 1], o[cb][4 * q + 3]};
+    if (half == 0) {
+        pm[0] = st.m;
+        pm[1] = l;
     }
 }
 
@@ -515,24 +448,23 @@ int check_layer(const akv_cache_layer *c, const char *what) {
     return AKV_OK;
 }
 
-// How a call is cut up: the rows of a KV head into groups of 16 or 32 (one or two matrix columns a lane), the planes into splits
-// of whole tiles.
+// How a call is cut up: the rows of a KV head into groups of 32, 64 or 128 (4, 2 or 1 parts), the planes into splits of whole rounds.
 struct TreePlan {
-    int nt, tok, groups, plane_splits, tiles_per_split, splits;
+    int parts, tokens, groups, plane_splits, tokens_per_split, splits;
 };
-static TreePlan tree_plan(int bsz, int n_kv_heads, int rows, int bound) {
+static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int bound) {
     TreePlan p;
-    p.nt = rows > 16 ? 2 : 1;
-    p.tok = p.nt == 2 ? 128 : 256;
-    p.groups = (rows + 16 * p.nt - 1) / (16 * p.nt);
-    const int flushed = bound / kRest * kRest, tiles = (flushed + p.tok - 1) / p.tok;
+    p.parts = rows > 64 ? 1 : (rows > 32 ? 2 : 4);
+    p.tokens = p.parts == 4 ? 128 : p.parts * (head_dim == 256 ? 32 : 64);
+    p.groups = (rows + 128 / p.parts - 1) / (128 / p.parts);
+    const int flushed = bound / kRest * kRest, rounds = (flushed + p.tokens - 1) / p.tokens;
     const int64_t units = (int64_t)bsz * n_kv_heads * p.groups;
-    int64_t want = (512 + units - 1) / units;                 // two workgroups per compute unit
-    const int64_t most = (tiles + 3) / 4;                     // four waves take a tile each
-    if (want > most) want = most;
+    AKV_TUNE("AKV_TUNE_TREE_WGS", forced);
+    int64_t want = ((has_forced ? forced : 1024) + units - 1) / units;
+    if (want > rounds) want = rounds;
     if (want < 1) want = 1;
-    p.tiles_per_split = tiles > 0 ? (int)((tiles + want - 1) / want) : 1;
-    p.plane_splits = (tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+    p.tokens_per_split = rounds > 0 ? (int)((rounds + want - 1) / want) * p.tokens : p.tokens;
+    p.plane_splits = (flushed + p.tokens_per_split - 1) / p.tokens_per_split;
     p.splits = p.plane_splits + 1;
     return p;
 }
@@ -541,15 +473,17 @@ template <int D, int KB>
 static void launch_tree(const TreeArgs &a, const TreePlan &p, bool cap, hipStream_t st) {
     const dim3 grid(p.splits, a.c.n_kv_heads * p.groups, a.c.bsz);
     const bool alibi = a.slopes != nullptr;
-#define AKV_TREE(TPL, NT, CAP, ALIBI) hipLaunchKernelGGL((tree_kernel<D, KB, TPL, NT, CAP, ALIBI>), grid, dim3(256), 0, st, a)
-#define AKV_TREE_NT(TPL, NT)                                                                                          \
-    do {                                                                                                              \
-        if (cap) { if (alibi) AKV_TREE(TPL, NT, true, true); else AKV_TREE(TPL, NT, true, false); }                   \
-        else { if (alibi) AKV_TREE(TPL, NT, false, true); else AKV_TREE(TPL, NT, false, false); }                     \
+    constexpr int BN = D == 256 ? 32 : 64;
+#define AKV_TREE(PARTS, BN, CAP, ALIBI) hipLaunchKernelGGL((tree_kernel<D, KB, PARTS, BN, CAP, ALIBI>), grid, dim3(256), 0, st, a)
+#define AKV_TREE_PARTS(PARTS, BN)                                                                                         \
+    do {                                                                                                                  \
+        if (cap) { if (alibi) AKV_TREE(PARTS, BN, true, true); else AKV_TREE(PARTS, BN, true, false); }                   \
+        else { if (alibi) AKV_TREE(PARTS, BN, false, true); else AKV_TREE(PARTS, BN, false, false); }                     \
     } while (0)
-    if (p.nt == 2) AKV_TREE_NT(8, 2);
-    else AKV_TREE_NT(16, 1);
-#undef AKV_TREE_NT
+    if (p.parts == 4) AKV_TREE_PARTS(4, 32);
+    else if (p.parts == 2) AKV_TREE_PARTS(2, BN);
+    else AKV_TREE_PARTS(1, BN);
+#undef AKV_TREE_PARTS
 #undef AKV_TREE
     hipLaunchKernelGGL(tree_combine_kernel<D>, dim3(a.rows, a.c.n_kv_heads, a.c.bsz), dim3(D), 0, st, a);
 }
@@ -559,7 +493,7 @@ static void launch_tree(const TreeArgs &a, const TreePlan &p, bool cap, hipStrea
 extern "C" size_t akv_tree_attention_workspace_bytes(int bsz, int n_q_heads, int n_kv_heads, int head_dim, int n_drafts, int len_bound) {
     if (bsz < 1 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || head_dim < 1 || n_drafts < 1 || n_drafts > 64 || len_bound < 0) return 0;
     const int rows = n_q_heads / n_kv_heads * n_drafts;
-    const akv::TreePlan p = akv::tree_plan(bsz, n_kv_heads, rows, len_bound);
+    const akv::TreePlan p = akv::tree_plan(bsz, n_kv_heads, head_dim, rows, len_bound);
     return (size_t)bsz * n_kv_heads * p.splits * rows * (head_dim + 2) * sizeof(float);
 }
 
@@ -588,8 +522,8 @@ extern "C" int akv_tree_attention(const akv_cache_layer *layer, const uint8_t *q
     a.parts = static_cast<float *>(workspace);
     a.T = n_drafts; a.Hq = n_q_heads; a.G = n_q_heads / layer->n_kv_heads; a.rows = a.T * a.G;
     a.form = akv::score_form(scale, softcap);
-    const akv::TreePlan p = akv::tree_plan(layer->bsz, layer->n_kv_heads, a.rows, len_bound);
-    a.plane_splits = p.plane_splits; a.tiles_per_split = p.tiles_per_split; a.splits = p.splits;
+    const akv::TreePlan p = akv::tree_plan(layer->bsz, layer->n_kv_heads, layer->head_dim, a.rows, len_bound);
+    a.plane_splits = p.plane_splits; a.tokens_per_split = p.tokens_per_split; a.splits = p.splits;
     AKV_REQUIRE((int64_t)layer->n_kv_heads * p.groups <= 65535, "tree_attention: too many rows");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool cap = softcap > 0.f;
