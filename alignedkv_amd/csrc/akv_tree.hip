@@ -46,11 +46,12 @@ struct Raw16 {
     u32x4 h;
     u32x2 m, l;
 };
-__device__ __forceinline__ Raw16 load_raw16(__amdgpu_buffer_rsrc_t rh, __amdgpu_buffer_rsrc_t rm, __amdgpu_buffer_rsrc_t rl, int off, bool in) {
+// (off: of the high bytes; kSkip and a little beyond it are out of every range, halved too)
+__device__ __forceinline__ Raw16 load_raw16(__amdgpu_buffer_rsrc_t rh, __amdgpu_buffer_rsrc_t rm, __amdgpu_buffer_rsrc_t rl, u32 off) {
     Raw16 r;
-    r.h = __builtin_amdgcn_raw_buffer_load_b128(rh, in ? off : kSkip, 0, 0);
-    r.m = __builtin_amdgcn_raw_buffer_load_b64(rm, in ? off >> 1 : kSkip, 0, 0);
-    r.l = __builtin_amdgcn_raw_buffer_load_b64(rl, in ? off >> 1 : kSkip, 0, 0);
+    r.h = __builtin_amdgcn_raw_buffer_load_b128(rh, (int)off, 0, 0);
+    r.m = __builtin_amdgcn_raw_buffer_load_b64(rm, (int)(off >> 1), 0, 0);
+    r.l = __builtin_amdgcn_raw_buffer_load_b64(rl, (int)(off >> 1), 0, 0);
     return r;
 }
 
@@ -79,7 +80,7 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
     }
 }
 
-// grid (splits, Hkv * row groups, B), 256 threads.  Split s < plane_splits: tiles of the planes; the last split: the rest buffer and the
+// grid: a workgroup per split, row group, KV head and sequence (see unit below); 256 threads.  Split s < plane_splits: tiles of the planes; the last split: the rest buffer and the
 // drafts.  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
 // unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
 // 128 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
@@ -96,7 +97,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     __shared__ int odd_tile[PARTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_index(), half = lane >> 5, part = wave / WAVES, part_tid = tid & (64 * WAVES - 1);
     const int groups = (a.rows + ROWS - 1) / ROWS;
-    const int split = blockIdx.x, hkv = blockIdx.y / groups, rg = blockIdx.y - hkv * groups, b = blockIdx.z;
+    // Workgroups are dealt out to the 8 XCDs in turn: the row groups of a stretch of the planes are 8 apart, so that one XCD's L2 serves
+    // them all.
+    const int unit = (int)(blockIdx.x / 8 / groups) * 8 + (int)(blockIdx.x % 8), rg = blockIdx.x / 8 % groups;
+    if (unit >= a.splits * a.c.n_kv_heads * a.c.bsz) return;
+    const int split = unit % a.splits, hkv = unit / a.splits % a.c.n_kv_heads, b = unit / a.splits / a.c.n_kv_heads;
     const int n = cached_tokens(a, b), flushed = n / kRest * kRest, n_rest = n - flushed, total = n_rest + a.T;
     const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv;
     const int row = rg * ROWS + (wave % WAVES) * 32 + (lane & 31), row_c = min(row, a.rows - 1), g = row_c / a.T, t = row_c - g * a.T;
@@ -106,50 +111,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     // the planes: this thread's pieces of a round
     const int first = split * a.tokens_per_split, end = tail ? 0 : min(first + a.tokens_per_split, flushed);
     Raw16 kr[UNITS], vr[UNITS];
+    // Piece u of a thread lies a constant behind piece 0, in memory and in LDS: four addresses stay in registers.
+    constexpr int kChStep = 256 * 16 / TT, kTokStep = 256 * 16 / D;      // channels / tokens from piece to piece
+    static_assert(kChStep % 16 == 0 && kTokStep % 16 == 0, "rows 16 apart are laid out alike");
+    const int k_tok = tid % (TT / 16) * 16, k_ch = tid / (TT / 16), v_c16 = tid % (D / 16), v_tok = tid / (D / 16);
+    int k_lds = k_tok / BN * kPart + key_byte<BN>(k_ch, k_tok % BN / 8);                                // the other half: ^ 16
+    int v_lds = PARTS * kPart + v_tok / BN * kPart + tile_byte<D>(place(v_tok % BN), 2 * v_c16);
+    int v_off = v_tok * D + v_c16 * 16;
     auto request_k = [&](int j0) {
         const int64_t blk = bh * a.c.n_max_blocks + j0 / KB;
-        const int blocks = min(KB == 64 ? TT / 64 + (TT < 64) : 1, a.c.n_max_blocks - j0 / KB);
+        const int blocks = min(KB == 64 && TT > 64 ? TT / 64 : 1, a.c.n_max_blocks - j0 / KB);
         const auto rh = make_rsrc(a.c.k_first_8 + blk * (D * KB), blocks * D * KB);
         const auto rm = make_rsrc(a.c.k_mid_4 + blk * (D * KB / 2), blocks * D * KB / 2);
         const auto rl = make_rsrc(a.c.k_last_4 + blk * (D * KB / 2), blocks * D * KB / 2);
+        const int in = j0 % KB + k_tok;
+        const u32 off = j0 + k_tok < end ? in / KB * (D * KB) + k_ch * KB + in % KB : kSkip;
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int id = u * 256 + tid, tok = id % (TT / 16) * 16, ch = id / (TT / 16), in = j0 % KB + tok;
-            kr[u] = load_raw16(rh, rm, rl, in / KB * (D * KB) + ch * KB + in % KB, j0 + tok < end);
-        }
+        for (int u = 0; u < UNITS; ++u) kr[u] = load_raw16(rh, rm, rl, off + u * (kChStep * KB));
     };
     auto request_v = [&](int j0) {
         const int64_t r0 = bh * a.c.max_seq_len + j0;
-        const int rows = end - j0;
-        const auto rh = make_rsrc(a.c.v_first_8 + r0 * D, min(rows, TT) * D);
-        const auto rm = make_rsrc(a.c.v_mid_4 + r0 * (D / 2), min(rows, TT) * D / 2);
-        const auto rl = make_rsrc(a.c.v_last_4 + r0 * (D / 2), min(rows, TT) * D / 2);
+        const int rows = min(end - j0, TT);                   // (rows behind them are out of range)
+        const auto rh = make_rsrc(a.c.v_first_8 + r0 * D, rows * D);
+        const auto rm = make_rsrc(a.c.v_mid_4 + r0 * (D / 2), rows * D / 2);
+        const auto rl = make_rsrc(a.c.v_last_4 + r0 * (D / 2), rows * D / 2);
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int id = u * 256 + tid, c16 = id % (D / 16), tok = id / (D / 16);
-            vr[u] = load_raw16(rh, rm, rl, tok * D + c16 * 16, tok < rows);
-        }
+        for (int u = 0; u < UNITS; ++u) vr[u] = load_raw16(rh, rm, rl, v_off + u * (kTokStep * D));
     };
-    auto put_k = [&]() {
+    auto put = [&](int at, int step, const Raw16 (&raw)[UNITS]) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const int id = u * 256 + tid, tok = id % (TT / 16) * 16, ch = id / (TT / 16);
-            uint8_t *to = lds + tok / BN * kPart;
-            *reinterpret_cast<u32x4 *>(to + key_byte<BN>(ch, tok % BN / 8)) = rebuild8(kr[u].h.x, kr[u].h.y, kr[u].m.x, kr[u].l.x);
-            *reinterpret_cast<u32x4 *>(to + key_byte<BN>(ch, tok % BN / 8 + 1)) = rebuild8(kr[u].h.z, kr[u].h.w, kr[u].m.y, kr[u].l.y);
-        }
-    };
-    auto put_v = [&]() {
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const int id = u * 256 + tid, c16 = id % (D / 16), tok = id / (D / 16);
-            uint8_t *to = lds + PARTS * kPart + tok / BN * kPart;
-            *reinterpret_cast<u32x4 *>(to + tile_byte<D>(place(tok % BN), 2 * c16)) = rebuild8(vr[u].h.x, vr[u].h.y, vr[u].m.x, vr[u].l.x);
-            *reinterpret_cast<u32x4 *>(to + tile_byte<D>(place(tok % BN), 2 * c16 + 1)) = rebuild8(vr[u].h.z, vr[u].h.w, vr[u].m.y, vr[u].l.y);
+            *reinterpret_cast<u32x4 *>(lds + at + u * step) = rebuild8(raw[u].h.x, raw[u].h.y, raw[u].m.x, raw[u].l.x);
+            *reinterpret_cast<u32x4 *>(lds + (at ^ 16) + u * step) = rebuild8(raw[u].h.z, raw[u].h.w, raw[u].m.y, raw[u].l.y);
         }
     };
     // (V of a round is asked for behind its K: both at once do not fit beside the sums, except where a wave has a SIMD to itself)
-    constexpr bool kAhead = D == 64;
+    constexpr bool kAhead = !(D == 256 && PARTS == 4);
     if (first < end) {
         request_k(first);
         if constexpr (kAhead) request_v(first);
@@ -176,8 +173,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
 
     for (int j0 = first; j0 < end; j0 += TT) {
         at.pin();
-        asm volatile("" : "+v"(k_at0), "+v"(k_at1));
-        put_k();
+        asm volatile("" : "+v"(k_at0), "+v"(k_at1), "+v"(k_lds), "+v"(v_lds), "+v"(v_off));
+        put(k_lds, kChStep * BN * 2, kr);
         const int next = j0 + TT;
         if constexpr (kAhead) {
             if (next < end) request_k(next);
@@ -195,7 +192,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
             factor = modify_block<CAP, TB>(x, a.form);
             if constexpr (ALIBI) {
                 // every cached token lies before the row: the distance is linear in the token
-                const float s = neg_slope / factor;
+                const float s = neg_slope * __builtin_amdgcn_rcpf(factor);       // (the same in every lane; times factor again: 1 ulp of the bias)
                 shift = -neg_slope * (float)(jp + 4 * half - pos);
 #pragma unroll
                 for (int tb = 0; tb < TB; ++tb)
@@ -204,7 +201,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
             }
             tile_softmax<D, BN>(x, factor, shift, st, o, p);
         }
-        put_v();
+        put(v_lds, kTokStep * D * 2, vr);
         if (next < end) {
             if constexpr (kAhead) request_v(next);
             else request_k(next);
@@ -471,7 +468,7 @@ static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int b
 
 template <int D, int KB>
 static void launch_tree(const TreeArgs &a, const TreePlan &p, bool cap, hipStream_t st) {
-    const dim3 grid(p.splits, a.c.n_kv_heads * p.groups, a.c.bsz);
+    const dim3 grid((u32)(((int64_t)p.splits * a.c.n_kv_heads * a.c.bsz + 7) / 8 * 8 * p.groups));
     const bool alibi = a.slopes != nullptr;
     constexpr int BN = D == 256 ? 32 : 64;
 #define AKV_TREE(PARTS, BN, CAP, ALIBI) hipLaunchKernelGGL((tree_kernel<D, KB, PARTS, BN, CAP, ALIBI>), grid, dim3(256), 0, st, a)
@@ -524,7 +521,7 @@ extern "C" int akv_tree_attention(const akv_cache_layer *layer, const uint8_t *q
     a.form = akv::score_form(scale, softcap);
     const akv::TreePlan p = akv::tree_plan(layer->bsz, layer->n_kv_heads, layer->head_dim, a.rows, len_bound);
     a.plane_splits = p.plane_splits; a.tokens_per_split = p.tokens_per_split; a.splits = p.splits;
-    AKV_REQUIRE((int64_t)layer->n_kv_heads * p.groups <= 65535, "tree_attention: too many rows");
+    AKV_REQUIRE(((int64_t)p.splits * layer->n_kv_heads * layer->bsz + 8) * p.groups < (1ll << 31), "tree_attention: too many rows");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool cap = softcap > 0.f;
     if (layer->k_block == 64) {
