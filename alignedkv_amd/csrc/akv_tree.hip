@@ -81,7 +81,7 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
 }
 
 // grid: a workgroup per split, row group, KV head and sequence (see unit below); 256 threads.  Split s < plane_splits: tiles of the planes; the last split: the rest buffer and the
-// drafts.  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
+// drafts (behind its share of the planes, if it has one).  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
 // unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
 // 128 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
 // tree_combine_kernel.
@@ -105,11 +105,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     const int n = cached_tokens(a, b), flushed = n / kRest * kRest, n_rest = n - flushed, total = n_rest + a.T;
     const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv;
     const int row = rg * ROWS + (wave % WAVES) * 32 + (lane & 31), row_c = min(row, a.rows - 1), g = row_c / a.T, t = row_c - g * a.T;
-    const bool tail = split == a.plane_splits;
+    const bool tail = split == a.splits - 1;
     uint8_t *kt = lds + part * kPart, *vt = lds + PARTS * kPart + part * kPart;
 
     // the planes: this thread's pieces of a round
-    const int first = split * a.tokens_per_split, end = tail ? 0 : min(first + a.tokens_per_split, flushed);
+    const int first = split * a.tokens_per_split, end = split < a.plane_splits ? min(first + a.tokens_per_split, flushed) : 0;
     Raw16 kr[UNITS], vr[UNITS];
     // Piece u of a thread lies a constant behind piece 0, in memory and in LDS: four addresses stay in registers.
     constexpr int kChStep = 256 * 16 / TT, kTokStep = 256 * 16 / D;      // channels / tokens from piece to piece
@@ -322,25 +322,39 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     }
 }
 
-// One workgroup of D threads per query row: joins the splits in order.
+// Joins the splits of a row in order: D / 4 lanes a row, four channels a lane, four splits' sums requested at a time.
 template <int D>
-__global__ __launch_bounds__(D) void tree_combine_kernel(TreeArgs a) {
-    const int row = blockIdx.x, hkv = blockIdx.y, b = blockIdx.z, ch = threadIdx.x;
-    const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv;
-    const float *po = a.parts + bh * a.splits * (int64_t)a.rows * D + (int64_t)row * D + ch;
-    const float *pm = a.parts + (int64_t)a.c.bsz * a.c.n_kv_heads * a.splits * a.rows * D + bh * a.splits * (int64_t)a.rows * 2 + row * 2;
-    float m = kNegInf;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, pm[(int64_t)s * a.rows * 2]);
-    float o = 0.f, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float ms = pm[(int64_t)s * a.rows * 2];
-        const float f = ms == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-        o = fmaf(po[(int64_t)s * a.rows * D], f, o);
-        l = fmaf(pm[(int64_t)s * a.rows * 2 + 1], f, l);
+__global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
+    constexpr int LANES = D / 4, ROWS = 256 / LANES;
+    const int row = blockIdx.x * ROWS + threadIdx.x / LANES, hkv = blockIdx.y, b = blockIdx.z, ch = threadIdx.x % LANES * 4;
+    if (row >= a.rows) return;
+    const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv, step = (int64_t)a.rows * D;
+    const float *po = a.parts + bh * a.splits * step + (int64_t)row * D + ch;
+    const f32x2 *pm = reinterpret_cast<const f32x2 *>(a.parts + (int64_t)a.c.bsz * a.c.n_kv_heads * a.splits * step) + bh * a.splits * a.rows + row;
+    float m = kNegInf, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        f32x4 x[4];
+        f32x2 ml[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = min(s0 + i, a.splits - 1);
+            x[i] = *reinterpret_cast<const f32x4 *>(po + s * step);
+            ml[i] = pm[(int64_t)s * a.rows];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i >= a.splits) break;
+            const float top = fmaxf(m, ml[i].x);
+            const float f0 = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - top), f1 = ml[i].x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - top);
+            o = o * f0 + x[i] * f1;
+            l = l * f0 + ml[i].y * f1;
+            m = top;
+        }
     }
-    const float r = l == 0.f ? o : o / l;      // (a row that saw nothing: zero)
+    const float r = l == 0.f ? 1.f : 1.f / l;      // (a row that saw nothing: zeros)
     const int g = row / a.T, t = row - g * a.T;
-    reinterpret_cast<unsigned short *>(a.out)[(((int64_t)b * a.T + t) * a.Hq + hkv * a.G + g) * D + ch] = float_to_half_bits(r);
+    *reinterpret_cast<u32x2 *>(a.out + ((((int64_t)b * a.T + t) * a.Hq + hkv * a.G + g) * D + ch) * 2) = u32x2{pack_f16(o[0] * r, o[1] * r), pack_f16(o[2] * r, o[3] * r)};
 }
 
 // ---- commit of accepted drafts ---------------------------------------------------------------------------------------------------------
@@ -456,13 +470,17 @@ static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int b
     p.groups = (rows + 128 / p.parts - 1) / (128 / p.parts);
     const int flushed = bound / kRest * kRest, rounds = (flushed + p.tokens - 1) / p.tokens;
     const int64_t units = (int64_t)bsz * n_kv_heads * p.groups;
-    AKV_TUNE("AKV_TUNE_TREE_WGS", forced);
-    int64_t want = ((has_forced ? forced : 1024) + units - 1) / units;
+    // Workgroups in one round of the chip: two a compute unit (one with head_dim 256, which takes the registers of both).  Where the
+    // planes' traffic, not the arithmetic, is what a call waits for, fewer of them leave fewer sums to join: 16 drafts x 4 heads a KV head
+    // over 8 x 8150 tokens 50.3 us with 384 against 56.6 with 512; 64 drafts over 4 x 32768, which is arithmetic, 297 against 258.
+    const int aim = head_dim == 256 ? 256 : (p.parts == 1 ? 512 : 384);
+    int64_t want = (aim + units - 1) / units;
     if (want > rounds) want = rounds;
     if (want < 1) want = 1;
     p.tokens_per_split = rounds > 0 ? (int)((rounds + want - 1) / want) * p.tokens : p.tokens;
     p.plane_splits = (flushed + p.tokens_per_split - 1) / p.tokens_per_split;
-    p.splits = p.plane_splits + 1;
+    // the tail gets a workgroup of its own while there are compute units without one
+    p.splits = p.plane_splits + (p.plane_splits == 0 || units * (p.plane_splits + 1) <= 256 ? 1 : 0);
     return p;
 }
 
@@ -482,7 +500,7 @@ static void launch_tree(const TreeArgs &a, const TreePlan &p, bool cap, hipStrea
     else AKV_TREE_PARTS(1, BN);
 #undef AKV_TREE_PARTS
 #undef AKV_TREE
-    hipLaunchKernelGGL(tree_combine_kernel<D>, dim3(a.rows, a.c.n_kv_heads, a.c.bsz), dim3(D), 0, st, a);
+    hipLaunchKernelGGL(tree_combine_kernel<D>, dim3((a.rows + 1024 / D - 1) / (1024 / D), a.c.n_kv_heads, a.c.bsz), dim3(256), 0, st, a);
 }
 
 }  // namespace akv
