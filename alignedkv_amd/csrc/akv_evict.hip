@@ -72,41 +72,67 @@ __device__ __forceinline__ Choice make_choice(int n, int keep, int sinks, int re
     return c;
 }
 
-// One workgroup of 1024 per (sequence, KV head).  The `need`-th largest key is found by its digits, 11 + 11 + 10 bits, each from
-// a histogram in LDS; then every wave writes the chosen tokens of its stretch of the row behind those of the waves before it.
-__global__ __launch_bounds__(1024) void evict_select_kernel(const float *__restrict__ weights, int64_t w_b, int64_t w_h, const int *__restrict__ lens,
+// One workgroup per (sequence, KV head), of 1024 threads, or of 256 where the rows are short (their barriers are cheaper: 1024 tokens
+// 11.5 us against 14.8).  The `need`-th largest key is found by its digits, 11 + 11 + 10 bits, each from a
+// histogram in LDS; then the chosen tokens are written in order.  Token THREADS i + thread is this thread's i-th: the keys of the first
+// kHeld * THREADS tokens are read once and kept in registers (32000 tokens: 46 us with every pass reading them, latency, not
+// bytes), those of a longer row again in every pass.
+constexpr int kHeld = 32;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void evict_select_kernel(const float *__restrict__ weights, int64_t w_b, int64_t w_h, const int *__restrict__ lens,
                                                             int *__restrict__ kept, int *__restrict__ old_lens, int Hkv, int capacity, int keep, int sinks,
                                                             int recent) {
     __shared__ u32 hist[2048];
-    __shared__ int wave_tot[16], wave_eq[16];
+    constexpr int WAVES = THREADS / 64, BINS = 2048 / THREADS;
+    __shared__ int wave_tot[WAVES];
     __shared__ u32 digit_s;
     __shared__ int above_s;
     const int h = blockIdx.x % Hkv, b = blockIdx.x / Hkv, tid = threadIdx.x, lane = tid & 63, wave = wave_index();
     const Choice c = make_choice(max(0, min(lens[b], capacity)), keep, sinks, recent);
     int *out = kept + (int64_t)blockIdx.x * keep;
     if (h == 0 && tid == 0) old_lens[b] = c.n;
-    for (int i = c.have + tid; i < keep; i += 1024) out[i] = -1;
+    for (int i = c.have + tid; i < keep; i += THREADS) out[i] = -1;
     if (c.flushed <= keep) {
-        for (int i = tid; i < c.have; i += 1024) out[i] = i;
+        for (int i = tid; i < c.have; i += THREADS) out[i] = i;
         return;
     }
     const float *w = weights + b * w_b + h * w_h;
+    u32 held[kHeld];
+    // (behind the row's end: out of the descriptor's range, nothing is fetched)
+    const auto row = make_rsrc(w, (u32)min(c.flushed, kHeld * THREADS) * 4u);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = (u32)__builtin_amdgcn_raw_buffer_load_b32(row, (i * THREADS + tid) * 4, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = weight_key(__uint_as_float(held[i]));
+    // f(token, key, i) for every token of this thread
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (i * THREADS < c.flushed) f(i * THREADS + tid, held[i]);
+#pragma unroll 4
+        for (int j0 = kHeld * THREADS; j0 < c.flushed; j0 += THREADS) f(j0 + tid, weight_key(w[min(j0 + tid, c.flushed - 1)]));
+    };
+    const auto candidate = [&](int j) { return j >= c.lo && j < c.hi; };
     u32 prefix = 0;             // digits found so far
     int need = c.need;          // still to be taken among the keys that share them
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < 2048; i += 1024) hist[i] = 0;
+        for (int i = tid; i < 2048; i += THREADS) hist[i] = 0;
         __syncthreads();
-        for (int j = c.lo + tid; j < c.hi; j += 1024) {
-            const u32 k = weight_key(w[j]);
-            if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+        each([&](int j, u32 k) {
+            if (candidate(j) && (pass == 0 || (k >> (shift + bits)) == prefix)) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+        });
+        __syncthreads();
+        // thread i holds BINS bins below 2048 - BINS i: counts from the top
+        const int top = 2047 - BINS * tid;
+        int own[BINS], inc = 0;
+#pragma unroll
+        for (int k = 0; k < BINS; ++k) {
+            own[k] = (int)hist[top - k];
+            inc += own[k];
         }
-        __syncthreads();
-        // thread i holds bins 2046 - 2 i and 2047 - 2 i: counts from the top
-        const int top = 2047 - 2 * tid;
-        const int c1 = (int)hist[top], c0 = (int)hist[top - 1];
-        int inc = c0 + c1;
+        const int mine = inc;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(inc, d);
@@ -114,14 +140,15 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(const float *__restr
         }
         if (lane == 63) wave_tot[wave] = inc;
         __syncthreads();
-        int before = inc - c0 - c1;
-        for (int k = 0; k < wave; ++k) before += wave_tot[k];
-        if (before < need && need <= before + c1) {
-            digit_s = (u32)top;
-            above_s = before;
-        } else if (before + c1 < need && need <= before + c1 + c0) {
-            digit_s = (u32)(top - 1);
-            above_s = before + c1;
+        int before = lane < wave ? wave_tot[lane] : 0;
+        before = wave_sum_i32(before) + inc - mine;
+#pragma unroll
+        for (int k = 0; k < BINS; ++k) {
+            if (before < need && need <= before + own[k]) {
+                digit_s = (u32)(top - k);
+                above_s = before;
+            }
+            before += own[k];
         }
         __syncthreads();
         if (need > 0) {
@@ -130,41 +157,63 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(const float *__restr
         }
         __syncthreads();
     }
-    // need > 0: `prefix` is the smallest chosen key and `need` of the tokens that have it are chosen, the first ones
+    // need > 0: `prefix` is the smallest chosen key and `need` of the tokens that have it are chosen, the first ones: a token's place is the
+    // number of tokens before it that are chosen for sure plus the number of equal ones before it, at most `need`.
+    // Token THREADS r + 64 wave + lane: in order of r, then the wave, then the lane.  Eight rounds at a time.
     const bool any = c.need > 0;
-    const int per = (c.flushed + 1023) / 1024 * 64, first = wave * per, end = min(first + per, c.flushed);
-    int gt = 0, eq = 0;
-    for (int j0 = first; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        const bool in = j < end, must = in && (j < c.lo || j >= c.hi), cand = in && !must && any;
-        const u32 k = cand ? weight_key(w[j]) : 0u;
-        gt += __popcll(__ballot(must || (cand && k > prefix)));
-        eq += __popcll(__ballot(cand && k == prefix));
-    }
-    if (lane == 0) {
-        wave_tot[wave] = gt;
-        wave_eq[wave] = eq;
-    }
-    __syncthreads();
-    int at = 0, eq_before = 0;
-    for (int k = 0; k < wave; ++k) {
-        at += wave_tot[k] + max(0, min(wave_eq[k], need - eq_before));
-        eq_before += wave_eq[k];
-    }
-    for (int j0 = first; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        const bool in = j < end, must = in && (j < c.lo || j >= c.hi), cand = in && !must && any;
-        const u32 k = cand ? weight_key(w[j]) : 0u;
-        const unsigned long long below = (1ull << lane) - 1, same = __ballot(cand && k == prefix);
-        const bool tie = cand && k == prefix && eq_before + __popcll(same & below) < need;
-        const bool take = must || (cand && k > prefix) || tie;
-        const unsigned long long all = __ballot(take);
-        if (take) {
-            const int slot = at + __popcll(all & below);
-            if (slot < keep) out[slot] = j;
+    const unsigned long long below = (1ull << lane) - 1;
+    __shared__ u32 counts[8 * WAVES];          // [round][wave]: chosen for sure, equal << 16
+    int sure_before = 0, eq_before = 0;
+    const auto rounds8 = [&](int j0, const u32 (&key)[8]) {
+        unsigned long long sure[8], same[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int j = j0 + r * THREADS + tid;
+            const bool in = j < c.flushed, cand = in && candidate(j) && any;
+            sure[r] = __ballot((in && !candidate(j)) || (cand && key[r] > prefix));
+            same[r] = __ballot(cand && key[r] == prefix);
+            if (lane == 0) counts[r * WAVES + wave] = (u32)__popcll(sure[r]) | (u32)__popcll(same[r]) << 16;
         }
-        at += __popcll(all);
-        eq_before += __popcll(same);
+        __syncthreads();
+        // every wave sums the counts up: two entries a lane
+        const bool real = lane < 4 * WAVES;
+        const u32 v0 = real ? counts[2 * lane] : 0u, v1 = real ? counts[2 * lane + 1] : 0u;
+        u32 inc = v0 + v1;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const u32 o = (u32)__shfl_up((int)inc, d);
+            if (lane >= d) inc += o;
+        }
+        const u32 excl = inc - v0 - v1 + (wave & 1 ? v0 : 0u);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const u32 before = (u32)__builtin_amdgcn_readlane((int)excl, r * (WAVES / 2) + (wave >> 1));
+            const int s0 = sure_before + (int)(before & 0xFFFFu), e0 = eq_before + (int)(before >> 16) + __popcll(same[r] & below);
+            const bool tie = (same[r] >> lane) & 1;
+            if (((sure[r] >> lane) & 1) || (tie && e0 < need)) {
+                const int slot = s0 + __popcll(sure[r] & below) + min(e0, need);
+                if (slot < keep) out[slot] = j0 + r * THREADS + tid;
+            }
+        }
+        const u32 all = (u32)__builtin_amdgcn_readlane((int)inc, 63);
+        sure_before += (int)(all & 0xFFFFu);
+        eq_before += (int)(all >> 16);
+        __syncthreads();
+    };
+#pragma unroll
+    for (int q = 0; q < kHeld / 8; ++q) {
+        if (q * (8 * THREADS) >= c.flushed) break;
+        u32 key[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) key[r] = held[q * 8 + r];
+        rounds8(q * (8 * THREADS), key);
+    }
+#pragma unroll 1
+    for (int j0 = kHeld * THREADS; j0 < c.flushed; j0 += 8 * THREADS) {
+        u32 key[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) key[r] = weight_key(w[min(j0 + r * THREADS + tid, c.flushed - 1)]);
+        rounds8(j0, key);
     }
 }
 
@@ -179,80 +228,162 @@ struct MoveArgs {
     int keep, sinks, recent, w_cap, only_moved;   // only_moved: sequences that keep everything stay as they are
 };
 
-// grid (2 * keep / 64, B * Hkv), 256 threads: 64 kept tokens of one KV head, keys (even blockIdx.x) or values (odd).
-__global__ __launch_bounds__(256) void evict_planes_kernel(MoveArgs a) {
-    __shared__ int src[kUnit];
-    const int H = a.from.n_kv_heads, D = a.from.head_dim, bh = blockIdx.y, b = bh / H, i0 = (blockIdx.x >> 1) * kUnit, tid = threadIdx.x;
-    const Choice c = make_choice(a.old_lens[b], a.keep, a.sinks, a.recent);
-    if (i0 >= c.have || (a.only_moved && c.flushed <= a.keep)) return;
-    if (tid < kUnit) src[tid] = max(0, min(a.kept ? a.kept[(int64_t)bh * a.keep + i0 + tid] : i0 + tid, c.flushed - 1));
-    __syncthreads();
-    if (blockIdx.x & 1) {
-        const int64_t from = (int64_t)bh * a.from.max_seq_len, to = (int64_t)bh * a.to.max_seq_len + i0;
-        const int cpr = D / 16;       // 16-byte pieces of a row of high bytes
-        for (int id = tid; id < kUnit * cpr; id += 256) {
-            const int r = id / cpr, p = id - r * cpr;
-            *reinterpret_cast<u32x4 *>(a.to.v_first_8 + (to + r) * D + p * 16) = *reinterpret_cast<const u32x4 *>(a.from.v_first_8 + (from + src[r]) * D + p * 16);
-        }
-        for (int id = tid; id < kUnit * cpr; id += 256) {
-            const int r = id / cpr, p = id - r * cpr;
-            *reinterpret_cast<u32x2 *>(a.to.v_mid_4 + (to + r) * (D / 2) + p * 8) = *reinterpret_cast<const u32x2 *>(a.from.v_mid_4 + (from + src[r]) * (D / 2) + p * 8);
-            *reinterpret_cast<u32x2 *>(a.to.v_last_4 + (to + r) * (D / 2) + p * 8) = *reinterpret_cast<const u32x2 *>(a.from.v_last_4 + (from + src[r]) * (D / 2) + p * 8);
-        }
-        return;
-    }
-    // keys: a thread takes four kept tokens of a channel
-    const int kb = a.from.k_block, r = (tid & 15) * 4;
-    const int64_t to = ((int64_t)bh * a.to.n_max_blocks + i0 / kb) * D * kb + i0 % kb + r;
-    int64_t from[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) from[t] = ((int64_t)bh * a.from.n_max_blocks + src[r + t] / kb) * D * kb + src[r + t] % kb;
-    for (int d = tid >> 4; d < D; d += 16) {
-        u32 hi = 0, mid = 0, last = 0;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int64_t at = from[t] + (int64_t)d * kb;
-            const u32 sh = at & 1 ? 0 : 4, place = (t >> 1) * 8 + (t & 1 ? 0 : 4);
-            hi |= (u32)a.from.k_first_8[at] << (8 * t);
-            mid |= ((a.from.k_mid_4[at >> 1] >> sh) & 15u) << place;
-            last |= ((a.from.k_last_4[at >> 1] >> sh) & 15u) << place;
-        }
-        *reinterpret_cast<u32 *>(a.to.k_first_8 + to + (int64_t)d * kb) = hi;
-        *reinterpret_cast<unsigned short *>(a.to.k_mid_4 + (to + (int64_t)d * kb) / 2) = (unsigned short)mid;
-        *reinterpret_cast<unsigned short *>(a.to.k_last_4 + (to + (int64_t)d * kb) / 2) = (unsigned short)last;
+// per_head = keep / 64 * (1 + D / 32) + rest chunks workgroups of 256 threads for each KV head.  The first keep / 64 workgroups of a KV head move the values of 64
+// kept tokens each, the next keep / 64 * D / 32 the keys of 64 kept tokens and 32 channels, the last ones everything else.
+constexpr int kRestChunk = 4096;       // weights a workgroup moves
+
+// Values: rows of D + D / 2 + D / 2 bytes, gathered 16 and 8 bytes a lane.
+__device__ __forceinline__ void move_values(const MoveArgs &a, int bh, int i0, const int *src) {
+    const int D = a.from.head_dim, tid = threadIdx.x, cpr = D / 16;
+    const int64_t from = (int64_t)bh * a.from.max_seq_len, to = (int64_t)bh * a.to.max_seq_len + i0;
+#pragma unroll 4
+    for (int id = tid; id < kUnit * cpr; id += 256) {
+        const int r = id / cpr, p = id - r * cpr;
+        const int64_t f = (from + src[r]) * D + p * 16, t = (to + r) * D + p * 16;
+        *reinterpret_cast<u32x4 *>(a.to.v_first_8 + t) = *reinterpret_cast<const u32x4 *>(a.from.v_first_8 + f);
+        *reinterpret_cast<u32x2 *>(a.to.v_mid_4 + t / 2) = *reinterpret_cast<const u32x2 *>(a.from.v_mid_4 + f / 2);
+        *reinterpret_cast<u32x2 *>(a.to.v_last_4 + t / 2) = *reinterpret_cast<const u32x2 *>(a.from.v_last_4 + f / 2);
     }
 }
 
-// grid B * Hkv, 256 threads: weights (kept ones, then the rest buffer's, zeros behind; in order, so that they may move within their
-// row), rest buffers, column maxima and lengths.
-__global__ __launch_bounds__(256) void evict_rest_kernel(MoveArgs a, int copy) {
-    const int H = a.from.n_kv_heads, D = a.from.head_dim, bh = blockIdx.x, b = bh / H, h = bh - b * H, tid = threadIdx.x;
-    const Choice c = make_choice(a.old_lens[b], a.keep, a.sinks, a.recent);
-    const int left = c.n - c.flushed + c.have;
-    if (copy) {
-        const int pieces = D / 8;
-        for (int id = tid; id < kUnit * pieces; id += 256) {
-            const int64_t at = (((int64_t)b * kUnit + id / pieces) * H + h) * D * 2 + (id % pieces) * 16;
-            *reinterpret_cast<u32x4 *>(a.to.restk + at) = *reinterpret_cast<const u32x4 *>(a.from.restk + at);
-            *reinterpret_cast<u32x4 *>(a.to.restv + at) = *reinterpret_cast<const u32x4 *>(a.from.restv + at);
+// Keys: a channel's tokens lie side by side, so a kept token is a byte here and a nibble there in 3 D places, and nearly every line
+// of a block that holds kept tokens is touched.  Blocks of 256 source tokens that hold any are brought into LDS whole (32 channels:
+// 16 KB, asynchronous, the next one while this one is searched); a lane owns a kept token, a wave eight channels: reading a byte a
+// lane out of one channel's row is free of bank conflicts, and the token's bytes stay in four registers until its block has come by.
+// Gathering the bytes from memory kept the address units busy instead: 217 us at 8 x 32000 tokens x 8 heads x 128 to 4096.
+__device__ __forceinline__ void move_keys(const MoveArgs &a, int bh, int i0, int ch0, const int *src, uint8_t *stage, uint8_t *done) {
+    const int D = a.from.head_dim, kb = a.from.k_block, tid = threadIdx.x, lane = tid & 63, wave = wave_index();
+    const int my = src[lane];
+    const int per = 256 / kb;                       // plane blocks of a stretch of 256 tokens
+    const int blocks = a.from.n_max_blocks;
+    const u32 lds0 = lds_address(stage) + wave * 1024;
+    // the next stretch that holds a kept token at or behind place i: uniform in the workgroup
+    const auto stretch = [&](int i) { return i < kUnit ? src[i] >> 8 : -1; };
+    const auto first_behind = [&](int s) { return (int)__popcll(__ballot((my >> 8) <= s)); };       // (kept tokens ascend)
+    auto request = [&](int s, int buf) {
+        // piece p (16 bytes of the high bytes) of the stretch: block p / (2 kb), channel, part; the nibble planes half as many
+        const int64_t blk = (int64_t)bh * blocks + (int64_t)s * per;
+        const int have = min(per, blocks - s * per);
+        const auto rh = make_rsrc(a.from.k_first_8 + blk * D * kb, (u32)(have * D * kb));
+        const auto rm = make_rsrc(a.from.k_mid_4 + blk * D * kb / 2, (u32)(have * D * kb / 2));
+        const auto rl = make_rsrc(a.from.k_last_4 + blk * D * kb / 2, (u32)(have * D * kb / 2));
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int byte = (c * 256 + tid) * 16, z = byte / (32 * kb), in = byte - z * (32 * kb);
+            load_to_lds(rh, lds0 + buf * 16384 + c * 4096, z < have ? z * D * kb + ch0 * kb + in : kSkip);
         }
-        for (int d = tid; d < D; d += 256) {
-            a.to.k_exp_column_max[(int64_t)bh * D + d] = a.from.k_exp_column_max[(int64_t)bh * D + d];
-            a.to.v_exp_column_max[(int64_t)bh * D + d] = a.from.v_exp_column_max[(int64_t)bh * D + d];
+        const int byte = tid * 16, z = byte / (16 * kb), in = byte - z * (16 * kb);
+        load_to_lds(rm, lds0 + buf * 16384 + 8192, z < have ? z * D * kb / 2 + ch0 * kb / 2 + in : kSkip);
+        load_to_lds(rl, lds0 + buf * 16384 + 12288, z < have ? z * D * kb / 2 + ch0 * kb / 2 + in : kSkip);
+    };
+    u32 hi[2] = {0u, 0u}, lo[2] = {0u, 0u};
+    int s = stretch(0), buf = 0;
+    request(s, 0);
+    while (s >= 0) {
+        const int next = stretch(first_behind(s));
+        wait_tile();
+        if (next >= 0) request(next, buf ^ 1);
+        if ((my >> 8) == s) {
+            const int z = (my & 255) / kb, slot = (my & 255) % kb;
+            const uint8_t *h = stage + buf * 16384 + z * (32 * kb) + wave * 8 * kb + slot, *m = stage + buf * 16384 + 8192 + z * (16 * kb) + wave * 4 * kb + (slot >> 1);
+            const int sh = slot & 1 ? 0 : 4;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                hi[k >> 2] |= (u32)h[k * kb] << (8 * (k & 3));
+                lo[k >> 2] |= ((((u32)m[k * kb / 2] >> sh) & 15u) << 4 | (((u32)m[4096 + k * kb / 2] >> sh) & 15u)) << (8 * (k & 3));
+            }
         }
+        buf ^= 1;
+        s = next;
     }
-    if (h == 0 && tid == 0) a.to.seq_lens[b] = left;
+    // token-major registers -> channel-major rows of 64 tokens
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        done[(wave * 8 + k) * kUnit + lane] = (uint8_t)(hi[k >> 2] >> (8 * (k & 3)));
+        done[2048 + (wave * 8 + k) * kUnit + lane] = (uint8_t)(lo[k >> 2] >> (8 * (k & 3)));
+    }
+    __syncthreads();
+    const int d = tid >> 3, r = (tid & 7) * 8;          // eight tokens of a channel
+    const u32x2 h8 = *reinterpret_cast<const u32x2 *>(done + d * kUnit + r), l8 = *reinterpret_cast<const u32x2 *>(done + 2048 + d * kUnit + r);
+    u32 mid = 0, last = 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const u32 x = q ? l8.y : l8.x;                  // low bytes of tokens 4 q ..: even ones to the high nibbles
+        const u32 m2 = (x & 0xF0u) | ((x >> 12) & 15u) | (((x >> 16) & 0xF0u) | (x >> 28)) << 8;
+        const u32 l2 = (x & 15u) << 4 | ((x >> 8) & 15u) | (((x >> 16) & 15u) << 4 | ((x >> 24) & 15u)) << 8;
+        mid |= m2 << (16 * q);
+        last |= l2 << (16 * q);
+    }
+    const int64_t to = (((int64_t)bh * a.to.n_max_blocks + i0 / kb) * D + ch0 + d) * kb + i0 % kb + r;
+    *reinterpret_cast<u32x2 *>(a.to.k_first_8 + to) = h8;
+    *reinterpret_cast<u32 *>(a.to.k_mid_4 + to / 2) = mid;
+    *reinterpret_cast<u32 *>(a.to.k_last_4 + to / 2) = last;
+}
+
+// Weights (kept ones, then the rest buffer's, zeros behind), rest buffers, column maxima and lengths.  Into another cache the chunks of a
+// row are independent; within a row (copy == 0) one workgroup goes through it in order.
+__device__ __forceinline__ void move_rest(const MoveArgs &a, const Choice &c, int bh, int chunk, int copy) {
+    const int H = a.from.n_kv_heads, D = a.from.head_dim, b = bh / H, h = bh - b * H, tid = threadIdx.x;
+    const int left = c.n - c.flushed + c.have;
+    if (chunk == 0) {
+        if (copy) {
+            const int pieces = D / 8;
+            for (int id = tid; id < kUnit * pieces; id += 256) {
+                const int64_t at = (((int64_t)b * kUnit + id / pieces) * H + h) * D * 2 + (id % pieces) * 16;
+                *reinterpret_cast<u32x4 *>(a.to.restk + at) = *reinterpret_cast<const u32x4 *>(a.from.restk + at);
+                *reinterpret_cast<u32x4 *>(a.to.restv + at) = *reinterpret_cast<const u32x4 *>(a.from.restv + at);
+            }
+            for (int d = tid; d < D; d += 256) {
+                a.to.k_exp_column_max[(int64_t)bh * D + d] = a.from.k_exp_column_max[(int64_t)bh * D + d];
+                a.to.v_exp_column_max[(int64_t)bh * D + d] = a.from.v_exp_column_max[(int64_t)bh * D + d];
+            }
+        }
+        if (h == 0 && tid == 0) a.to.seq_lens[b] = left;
+    }
     if (a.w_to == nullptr || (!copy && c.flushed <= a.keep)) return;
     const float *w = a.w_from + b * a.wf_b + h * a.wf_h;
     float *o = a.w_to + b * a.wt_b + h * a.wt_h;
-    for (int i0 = 0; i0 < left; i0 += 256) {
-        const int i = i0 + tid;
-        float x = 0.f;
-        if (i < left) x = w[i < c.have ? max(0, min(a.kept[(int64_t)bh * a.keep + i], c.flushed - 1)) : c.flushed + i - c.have];
-        __syncthreads();          // a weight never moves up its row: what later rounds read is not overwritten yet
-        if (i < left) o[i] = x;
+    const int first = copy ? chunk * kRestChunk : 0, end = copy ? min(first + kRestChunk, a.w_cap) : a.w_cap;
+    const int moved = min(left, end);
+    for (int i0 = first; i0 < moved; i0 += 2048) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = min(i0 + k * 256 + tid, moved - 1);
+            x[k] = w[i < c.have ? max(0, min(a.kept[(int64_t)bh * a.keep + i], c.flushed - 1)) : c.flushed + i - c.have];
+        }
+        if (!copy) __syncthreads();          // a weight never moves up its row: what later rounds read is not overwritten yet
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i0 + k * 256 + tid < moved) o[i0 + k * 256 + tid] = x[k];
     }
-    for (int i = left + tid; i < a.w_cap; i += 256) o[i] = 0.f;
+    for (int i = max(first, left) + tid; i < end; i += 256) o[i] = 0.f;
+}
+
+__global__ __launch_bounds__(256) void evict_rest_kernel(MoveArgs a) {
+    move_rest(a, make_choice(a.old_lens[blockIdx.x / a.from.n_kv_heads], a.keep, a.sinks, a.recent), blockIdx.x, 0, 0);
+}
+
+__global__ __launch_bounds__(256) void evict_move_kernel(MoveArgs a, int per_head, int with_rest, int copy) {
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[2 * 16384];
+    __shared__ __attribute__((aligned(16))) uint8_t done[4096];
+    __shared__ int src[kUnit];
+    // workgroups are dealt out to the 8 XCDs in turn: a KV head's go to one of them, where neighbouring tiles find the stretch they share in L2
+    const int bh = (int)(blockIdx.x / 8 / per_head) * 8 + (int)(blockIdx.x % 8), x = blockIdx.x / 8 % per_head;
+    if (bh >= a.from.bsz * a.from.n_kv_heads) return;
+    const int b = bh / a.from.n_kv_heads, tid = threadIdx.x, tiles = a.keep / kUnit, groups = a.from.head_dim / 32;
+    const Choice c = make_choice(a.old_lens[b], a.keep, a.sinks, a.recent);
+    if (x >= tiles * (1 + groups)) {
+        if (with_rest) move_rest(a, c, bh, x - tiles * (1 + groups), copy);
+        return;
+    }
+    // (the channel groups of a tile share their lines' neighbours: next to each other)
+    const int tile = x < tiles ? x : (x - tiles) / groups, i0 = tile * kUnit;
+    if (i0 >= c.have || (a.only_moved && c.flushed <= a.keep)) return;
+    if (tid < kUnit) src[tid] = max(0, min(a.kept ? a.kept[(int64_t)bh * a.keep + i0 + tid] : i0 + tid, c.flushed - 1));
+    __syncthreads();
+    if (x < tiles) move_values(a, bh, i0, src);
+    else move_keys(a, bh, i0, (x - tiles) % groups * 32, src, stage, done);
 }
 
 }  // namespace akv
@@ -303,7 +434,8 @@ extern "C" int akv_evict(const akv_cache_layer *from, const akv_cache_layer *to,
     AKV_REQUIRE(weights && kept, "evict: null pointer");
     AKV_REQUIRE(from->bsz == to->bsz && from->n_kv_heads == to->n_kv_heads && from->head_dim == to->head_dim && from->k_block == to->k_block,
                 "evict: the caches differ in batch, heads, head_dim or k_block");
-    AKV_REQUIRE(keep >= 64 && keep % 64 == 0, "evict: keep %d must be a positive multiple of 64", keep);
+    AKV_REQUIRE(keep >= 64 && keep % 64 == 0 && keep <= (1 << 20), "evict: keep %d must be a positive multiple of 64, at most 2^20", keep);
+    AKV_REQUIRE(((int64_t)from->bsz * from->n_kv_heads + 8) * (keep / 64 * 9 + 1 + weights_to_capacity / 4096) < (1ll << 31), "evict: too many tokens");
     AKV_REQUIRE(sinks >= 0 && recent >= 0 && (int64_t)sinks + recent <= keep, "evict: sinks %d and recent %d must fit into keep %d", sinks, recent, keep);
     const void *f[] = {from->k_first_8, from->k_mid_4, from->k_last_4, from->v_first_8, from->v_mid_4, from->v_last_4, from->k_exp_column_max,
                        from->v_exp_column_max, from->restk, from->restv, from->seq_lens};
@@ -330,11 +462,17 @@ extern "C" int akv_evict(const akv_cache_layer *from, const akv_cache_layer *to,
     a.wf_b = weights_stride_b; a.wf_h = weights_stride_h; a.wt_b = to_stride_b; a.wt_h = to_stride_h;
     a.keep = keep; a.sinks = sinks; a.recent = recent; a.w_cap = weights_to_capacity;
     a.only_moved = in_place;
-    hipLaunchKernelGGL(akv::evict_select_kernel, dim3(streams), dim3(1024), 0, st, weights, weights_stride_b, weights_stride_h, from->seq_lens, kept,
-                       static_cast<int *>(workspace), from->n_kv_heads, from->max_seq_len, keep, sinks, recent);
-    const dim3 grid(2 * (keep / 64), streams);
+#define AKV_SELECT(THREADS)                                                                                                             \
+    hipLaunchKernelGGL(akv::evict_select_kernel<THREADS>, dim3(streams), dim3(THREADS), 0, st, weights, weights_stride_b, weights_stride_h, \
+                       from->seq_lens, kept, static_cast<int *>(workspace), from->n_kv_heads, from->max_seq_len, keep, sinks, recent)
+    if (from->max_seq_len <= 256 * akv::kHeld) AKV_SELECT(256);
+    else AKV_SELECT(1024);
+#undef AKV_SELECT
+    const int moves = keep / 64 * (1 + from->head_dim / 32);
+    const auto grid = [&](int per_head) { return dim3((u32)((int64_t)((streams + 7) / 8 * 8) * per_head)); };
     if (!in_place) {
-        hipLaunchKernelGGL(akv::evict_planes_kernel, grid, dim3(256), 0, st, a);
+        const int chunks = weights_to ? (weights_to_capacity + akv::kRestChunk - 1) / akv::kRestChunk : 1;
+        hipLaunchKernelGGL(akv::evict_move_kernel, grid(moves + chunks), dim3(256), 0, st, a, moves + chunks, 1, 1);
     } else {
         uint8_t *w = static_cast<uint8_t *>(workspace) + p.lens_bytes;
         akv::MoveArgs m = a;
@@ -346,12 +484,14 @@ extern "C" int akv_evict(const akv_cache_layer *from, const akv_cache_layer *to,
         m.to.v_last_4 = m.to.v_mid_4 + p.v_first / 2;
         m.to.n_max_blocks = p.blocks;
         m.to.max_seq_len = keep;
-        hipLaunchKernelGGL(akv::evict_planes_kernel, grid, dim3(256), 0, st, m);
-        m.from = m.to;
-        m.to = a.to;
-        m.kept = nullptr;
-        hipLaunchKernelGGL(akv::evict_planes_kernel, grid, dim3(256), 0, st, m);
+        hipLaunchKernelGGL(akv::evict_move_kernel, grid(moves), dim3(256), 0, st, m, moves, 0, 0);
+        // back to the front of the cache's own planes, token i of the copy to place i; and the weights, within their rows
+        akv::MoveArgs back = m;
+        back.from = m.to;
+        back.to = a.to;
+        back.kept = nullptr;
+        hipLaunchKernelGGL(akv::evict_move_kernel, grid(moves), dim3(256), 0, st, back, moves, 0, 0);
+        hipLaunchKernelGGL(akv::evict_rest_kernel, dim3(streams), dim3(256), 0, st, a);
     }
-    hipLaunchKernelGGL(akv::evict_rest_kernel, dim3(streams), dim3(256), 0, st, a, in_place ? 0 : 1);
     return akv::check_launch("evict");
 }

@@ -362,60 +362,95 @@ __global__ __launch_bounds__(256, D == 256 || D * PARTS == 256 ? 1 : (D == 64 &&
 }
 
 // ---- the weight each token received -----------------------------------------------------------------------------------------------
-// w_j = sum over the heads g of the group and the rows i of the window of exp(s_ij - lse_i).  One wave owns 32 tokens of one
-// KV head: their keys stay in registers, the rows stream past them 32 at a time (q from L2: every wave of a KV head reads the
-// same rows), a lane sums its row's column of each product, and one reduction over the 32 rows ends it.  No atomics: the
-// sums' order is fixed.
+// w_j = sum over the heads g of the group and the rows i of the window of exp(s_ij - lse_i).  A workgroup owns 128 tokens of one KV
+// head, a wave 32 of them, whose keys stay in registers; the rows, head after head, stream past them through LDS, QR at a
+// time, two buffers filled by asynchronous loads (rows read by their lanes straight from memory, 32 lines a request, kept the address
+// units busy: 39 us at 2 x 8000 tokens, 64 rows of 32 heads).  A lane sums its row's column of each product, and one
+// reduction over the rows' lanes ends it.  No atomics: the order of a sum is fixed.
 template <int D, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256) void attention_weights_kernel(PromptArgs a, const float *__restrict__ lse, int window, float *__restrict__ w,
                                                                 int64_t w_b, int64_t w_h, int add) {
-    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-    const int hkv = blockIdx.y, b = blockIdx.z;
-    const int j0 = (blockIdx.x * 4 + wave_index()) * 32;
-    if (j0 >= a.S) return;
+    constexpr int QR = D == 256 ? 32 : 64, CPR = D / 8, kQ = QR * D * 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[128 * D * 2 > 2 * kQ ? 128 * D * 2 : 2 * kQ];       // the keys, then the rows
+    const int lane = threadIdx.x & 63, wave = wave_index(), half = lane >> 5, col = lane & 31;
+    const int hkv = blockIdx.y, b = blockIdx.z, jw = blockIdx.x * 128, j0 = jw + wave * 32;
     const int n = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
     const int prefix = a.prefix ? min(a.prefix[b], n) : 0;
     float sum[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-    if (j0 < n) {
+    int first = window > 0 ? max(0, n - window) : 0;
+    if (jw >= prefix) first = max(first, jw);           // rows before the tokens do not see them
+    const int blocks = jw < n ? (n - first + QR - 1) / QR : 0, rounds = blocks * a.G;
+    if (rounds > 0) {
+        const u32 lds0 = lds_address(lds) + wave * 1024;
+        const int my_row = threadIdx.x / CPR, my_chunk = threadIdx.x % CPR;
+        // rows j .. j + ROWS - 1 of a [token, head] matrix to LDS at byte `at`, the last row in place of those at and beyond n
+        auto bring = [&](const uint8_t *base, int64_t stride, int j, int rows_max, int at) {
+            const int rows = min(rows_max, n - j);
+            const auto rs = make_rsrc(base + (int64_t)j * stride, (u32)((rows - 1) * stride + D * 2));
+            for (int c = 0; c < rows_max * CPR / 256; ++c) {
+                const int r = my_row + c * (256 / CPR);
+                load_to_lds(rs, lds0 + at + c * 4096, (int)(min(r, rows - 1) * stride) + ((my_chunk ^ tile_swizzle<D>(r)) << 4));
+            }
+        };
+        bring(a.k + b * a.k_b + hkv * a.k_h, a.k_s, jw, 64, 0);
+        if (jw + 64 < n) bring(a.k + b * a.k_b + hkv * a.k_h, a.k_s, jw + 64, 64, 64 * D * 2);
+        wait_tile();
         f16x8 kf[D / 16];
-        const uint8_t *kp = a.k + b * a.k_b + (int64_t)min(j0 + col, n - 1) * a.k_s + hkv * a.k_h;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *reinterpret_cast<const f16x8 *>(kp + (2 * ks + half) * 16);
+        for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *reinterpret_cast<const f16x8 *>(lds + tile_byte<D>(wave * 32 + col, 2 * ks + half));
         int doc[16];
         if (a.docs) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) doc[r] = a.docs[(int64_t)b * a.S + min(j0 + 8 * (r >> 2) + 4 * half + (r & 3), n - 1)];
         }
-        int first = window > 0 ? max(0, n - window) : 0;
-        if (j0 >= prefix) first = max(first, j0);       // rows before the tokens do not see them
-        for (int g = 0; g < a.G; ++g) {
-            const int hq = hkv * a.G + g;
-            const float neg_slope = ALIBI ? a.slopes[hq] * -kLog2e : 0.f;
-            for (int i0 = first; i0 < n; i0 += 32) {
-                const int i = i0 + col, ic = min(i, n - 1);
-                const uint8_t *qp = a.q + b * a.q_b + (int64_t)ic * a.q_s + hq * a.q_h;
-                const float row_lse = lse[((int64_t)b * a.Hq + hq) * a.S + ic];
+        lds_barrier();
+        float row_lse[QR / 32], lse_next[QR / 32];
+        auto request = [&](int round, int buf) {
+            const int g = round / blocks, i0 = first + (round - g * blocks) * QR, hq = hkv * a.G + g;
+            bring(a.q + b * a.q_b + hq * a.q_h, a.q_s, i0, QR, buf * kQ);
+#pragma unroll
+            for (int tb = 0; tb < QR / 32; ++tb) lse_next[tb] = lse[((int64_t)b * a.Hq + hq) * a.S + min(i0 + tb * 32 + col, n - 1)];
+        };
+        request(0, 0);
+        int at_q = tile_byte<D>(col, half);
+        for (int round = 0; round < rounds; ++round) {
+            wait_tile();
+#pragma unroll
+            for (int tb = 0; tb < QR / 32; ++tb) row_lse[tb] = lse_next[tb] * kLog2e;
+            if (round + 1 < rounds) request(round + 1, (round + 1) & 1);
+            const int g = round / blocks, i0 = first + (round - g * blocks) * QR;
+            const float neg_slope = ALIBI ? a.slopes[hkv * a.G + g] * -kLog2e : 0.f;
+            const uint8_t *qt = lds + (round & 1) * kQ;
+            asm volatile("" : "+v"(at_q));
+#pragma unroll
+            for (int tb = 0; tb < QR / 32; ++tb) {
+                const int ib = i0 + tb * 32, i = ib + col;
+                if (ib >= n || (j0 > ib + 31 && j0 >= prefix) || j0 >= n) continue;
                 f32x16 x;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], *reinterpret_cast<const f16x8 *>(qp + (2 * ks + half) * 16), x, 0, 0, 0);
-                const int lim = i < n ? min(max(i, prefix - 1), n - 1) - j0 - 4 * half : -1;
-                const int my_doc = a.docs ? a.docs[(int64_t)b * a.S + ic] : 0;
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks], *reinterpret_cast<const f16x8 *>(qt + tb * 32 * D * 2 + (at_q ^ (ks << 5))), x, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int c = 8 * (r >> 2) + (r & 3);
-                    // the difference is formed before it is brought to base 2: both terms may be far larger than it
-                    float d;
-                    if constexpr (CAP) d = fmaf(a.form.c1, tanh_f32(x[r] * a.form.c0), -row_lse);
-                    else d = fmaf(x[r], a.form.c0, -row_lse);
-                    if constexpr (ALIBI) d = fmaf(neg_slope * kLn2, fabsf((float)(j0 + 4 * half + c - i)), d);
-                    const bool see = c <= lim && (!a.docs || (doc[r] == my_doc && my_doc >= 0));
-                    sum[r] += see ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.f;
+                    if constexpr (CAP) x[r] = fmaf(a.form.c1, tanh_f32(x[r] * a.form.c0), -row_lse[tb]);
+                    else x[r] = fmaf(x[r], a.form.c0, -row_lse[tb]);
+                    if constexpr (ALIBI) x[r] = fmaf(neg_slope, fabsf((float)(j0 + 4 * half + 8 * (r >> 2) + (r & 3) - i)), x[r]);
                 }
+                if (a.docs || ib + 32 > n || j0 + 32 > n || j0 + 31 > max(ib, prefix - 1)) {
+                    const int lim = i < n ? min(max(i, prefix - 1), n - 1) - j0 - 4 * half : -1;
+                    const int my_doc = a.docs ? a.docs[(int64_t)b * a.S + min(i, n - 1)] : 0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const bool see = 8 * (r >> 2) + (r & 3) <= lim && (!a.docs || (doc[r] == my_doc && my_doc >= 0));
+                        x[r] = see ? x[r] : kNegInf;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[r] += __builtin_amdgcn_exp2f(x[r]);
             }
         }
     }
@@ -544,10 +579,7 @@ extern "C" int akv_attention_weights(const akv_prompt_desc *desc, const float *l
     AKV_REQUIRE(lse && weights, "attention_weights: null pointer");
     AKV_REQUIRE(window >= 0, "attention_weights: window %d must be 0 (every row) or positive", window);
     AKV_REQUIRE(weights_stride_h >= a.S || a.Hkv == 1, "attention_weights: rows of %lld weights for %d tokens", (long long)weights_stride_h, a.S);
-    // differences against lse are formed in natural units
     const bool cap = desc->softcap > 0.f;
-    a.form.c0 = cap ? desc->scale / desc->softcap : desc->scale;
-    a.form.c1 = desc->softcap;
     const dim3 grid((a.S + 127) / 128, a.Hkv, a.B);
     const hipStream_t st = static_cast<hipStream_t>(stream);
 #define AKV_WEIGHTS(D, CAP, ALIBI)                                                                                             \

@@ -137,7 +137,7 @@ def test_evict_calls(lib, mem):
 
     says(lib, evict(w=None), "null pointer")
     says(lib, evict(kept=None), "null pointer")
-    for keep in (0, -64, 63, 100):
+    for keep in (0, -64, 63, 100, (1 << 20) + 64):
         says(lib, evict(keep=keep), f"keep {keep}")
     says(lib, evict(sinks=-1), "sinks -1")
     says(lib, evict(recent=-1), "recent -1")
