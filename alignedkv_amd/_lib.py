@@ -60,7 +60,7 @@ class StepDesc(ctypes.Structure):
 
 class PromptDesc(ctypes.Structure):
     """akv_prompt_desc of include/alignedkv.h."""
-    _fields_ = ([(n, _P) for n in ("q", "k", "v")] + [(n, c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+    _fields_ = ([(n, _P) for n in ("q", "k", "v")] + [(f"{n}_stride_{i}", c_int64) for n in "qkv" for i in "bsh"]
                 + [(n, _P) for n in ("slopes", "seq_lens", "prefix_lens", "documents")]
                 + [(n, _I) for n in ("bsz", "seqlen", "n_q_heads", "n_kv_heads", "head_dim")] + [("scale", c_float), ("softcap", c_float)])
 

@@ -360,87 +360,104 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
 // ---- commit of accepted drafts ---------------------------------------------------------------------------------------------------------
 // accepted[b]: indices of drafts, in order, up to the first one that is not in [0, T).  They are appended as decode steps would:
 // rest rows, a flush of 64 tokens into the planes when the rest buffer fills (at most one: 63 + 64 < 128), column maxima, lengths.
-constexpr int kCommitLayers = 16;      // layers per launch: their descriptors travel as kernel arguments
-struct CommitArgs {
-    akv_cache_layer c[kCommitLayers];
-    const uint8_t *k[kCommitLayers], *v[kCommitLayers];
-    const int *accepted;
-    int T, A;
+// What bounds it is latency: lengths, then indices, then rows, each a round trip, and few bytes behind them.  All layers of a
+// model go into one launch, their descriptors as kernel arguments.
+constexpr int kCommitLayers = 30;      // (4 KB of arguments)
+struct CommitLayer {
+    uint8_t *k_first_8, *k_mid_4, *k_last_4, *v_first_8, *v_mid_4, *v_last_4, *k_max, *v_max, *restk, *restv;
+    const int *seq_lens;
+    const uint8_t *k, *v;
+    int n_max_blocks, max_seq_len, k_block;
 };
+struct CommitArgs {
+    CommitLayer c[kCommitLayers];
+    const int *accepted;
+    int T, A, H;
+};
+static_assert(sizeof(CommitArgs) <= 4096, "kernel arguments");
 
-// grid (D / 16 * 2, B * Hkv, layers), 256 threads: a workgroup owns 16 channels of the keys (even blockIdx.x) or the values (odd) of one KV head.
+// How many of `accepted` are appended to a cache of n tokens: up to the first index outside [0, T), no further than the capacity.
+__device__ __forceinline__ int accepted_count(int index, int T, int n, int capacity) {
+    const unsigned long long ok = __ballot(index >= 0 && index < T);
+    return max(0, min(ok == ~0ull ? 64 : (int)__builtin_ctzll(~ok), capacity - n));
+}
+
+// grid (2, B * Hkv, layers), 256 threads: the keys (blockIdx.x 0) or the values of one KV head.
+template <int D>
 __global__ __launch_bounds__(256) void tree_commit_kernel(CommitArgs a) {
-    const akv_cache_layer &c = a.c[blockIdx.z];
-    __shared__ unsigned short tile[2 * kRest][16 + 2];
-    __shared__ int path[64];
-    __shared__ int count_s;
-    const bool is_v = blockIdx.x & 1;
-    const int ch0 = (blockIdx.x >> 1) * 16, D = c.head_dim, H = c.n_kv_heads;
-    const int b = blockIdx.y / H, h = blockIdx.y - b * H;
+    const CommitLayer &c = a.c[blockIdx.z];
+    constexpr int PITCH = D + 2, LANES = D / 4;          // a row of the tile in halves; threads to a row, four channels each
+    __shared__ __attribute__((aligned(16))) unsigned short tile[2 * kRest * PITCH];
+    const bool is_v = blockIdx.x;
+    const int H = a.H, b = blockIdx.y / H, h = blockIdx.y - b * H, tid = threadIdx.x, lane = tid & 63;
+    const int index = lane < a.A ? a.accepted[b * a.A + lane] : -1;
     const int n = max(0, c.seq_lens[b]), n_rest = n % kRest, flushed = n - n_rest;
-    if (threadIdx.x < 64) {
-        const int x = (int)threadIdx.x < a.A ? a.accepted[b * a.A + threadIdx.x] : -1;
-        path[threadIdx.x] = x;
-        const unsigned long long ok = __ballot(x >= 0 && x < a.T);
-        // no further than the cache's capacity
-        if (threadIdx.x == 0) count_s = max(0, min(ok == ~0ull ? 64 : (int)__builtin_ctzll(~ok), c.max_seq_len - n));
-    }
-    __syncthreads();
-    const int count = count_s;
+    const int count = accepted_count(index, a.T, n, c.max_seq_len);
     if (count == 0) return;
-    unsigned short *rest = reinterpret_cast<unsigned short *>(is_v ? c.restv : c.restk) + ((int64_t)b * kRest * H + h) * D + ch0;
-    const unsigned short *draft = reinterpret_cast<const unsigned short *>(is_v ? a.v[blockIdx.z] : a.k[blockIdx.z]) + ((int64_t)b * a.T * H + h) * D + ch0;
+    unsigned short *rest = reinterpret_cast<unsigned short *>(is_v ? c.restv : c.restk) + ((int64_t)b * kRest * H + h) * D;
+    const unsigned short *draft = reinterpret_cast<const unsigned short *>(is_v ? c.v : c.k) + ((int64_t)b * a.T * H + h) * D;
     const int64_t row = (int64_t)H * D;
     const int total = n_rest + count;
     const bool flush = total >= kRest;
-    // rows of the grown rest buffer: old ones only where they are flushed
-    for (int id = threadIdx.x; id < total * 16; id += 256) {
-        const int r = id >> 4, d = id & 15;
-        if (r >= n_rest) tile[r][d] = draft[path[r - n_rest] * row + d];
-        else if (flush) tile[r][d] = rest[r * row + d];
+    // the grown rest buffer: old rows only where they are flushed.  Its new rows go back to the rest buffer unless they are flushed,
+    // those behind the flush to its front.  (Rows read here are written below, behind the barrier.)
+    const int ch = tid % LANES * 4;
+    for (int r0 = flush ? 0 : n_rest; r0 < total; r0 += 256 / LANES) {
+        const int r = r0 + tid / LANES;
+        const int from = __shfl(index, max(0, min(r - n_rest, 63)));
+        if (r < total) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(r < n_rest ? rest + r * row + ch : draft + from * row + ch);
+            *reinterpret_cast<u32 *>(&tile[r * PITCH + ch]) = w.x;
+            *reinterpret_cast<u32 *>(&tile[r * PITCH + ch + 2]) = w.y;
+        }
     }
     __syncthreads();
-    uint8_t *colmax = (is_v ? c.v_exp_column_max : c.k_exp_column_max) + ((int64_t)b * H + h) * D + ch0;
-    if (threadIdx.x < 16) {
-        int mx = colmax[threadIdx.x];
-        for (int r = n_rest; r < total; ++r) mx = max(mx, (tile[r][threadIdx.x] >> 10) & 31);
-        colmax[threadIdx.x] = (uint8_t)mx;
+    uint8_t *colmax = (is_v ? c.v_max : c.k_max) + ((int64_t)b * H + h) * D;
+    if (tid < D) {
+        int mx = colmax[tid];
+        for (int r = n_rest; r < total; ++r) mx = max(mx, (tile[r * PITCH + tid] >> 10) & 31);
+        colmax[tid] = (uint8_t)mx;
     }
-    if (!flush) {
-        for (int id = threadIdx.x + n_rest * 16; id < total * 16; id += 256) rest[(id >> 4) * row + (id & 15)] = tile[id >> 4][id & 15];
-        return;
+    const int first = flush ? kRest : n_rest, shift = flush ? kRest : 0;
+    for (int r0 = first; r0 < total; r0 += 256 / LANES) {
+        const int r = r0 + tid / LANES;
+        if (r < total) {
+            const u32x2 w = {*reinterpret_cast<const u32 *>(&tile[r * PITCH + ch]), *reinterpret_cast<const u32 *>(&tile[r * PITCH + ch + 2])};
+            *reinterpret_cast<u32x2 *>(rest + (r - shift) * row + ch) = w;
+        }
     }
-    for (int id = threadIdx.x + kRest * 16; id < total * 16; id += 256) rest[((id >> 4) - kRest) * row + (id & 15)] = tile[id >> 4][id & 15];
+    if (!flush) return;
     const int64_t bh = (int64_t)b * H + h;
-    if (is_v) {
-        // token-major rows: 16 channels of a token are 16 + 8 + 8 bytes; a thread writes 4 channels
-        const int r = threadIdx.x >> 2, d = (threadIdx.x & 3) * 4;
-        const u32 w0 = tile[r][d], w1 = tile[r][d + 1], w2 = tile[r][d + 2], w3 = tile[r][d + 3];
-        const int64_t at = (bh * c.max_seq_len + flushed + r) * D + ch0 + d;
-        *reinterpret_cast<u32 *>(c.v_first_8 + at) = (w0 >> 8) | (w1 & 0xFF00u) | (w2 & 0xFF00u) << 8 | (w3 & 0xFF00u) << 16;
-        *reinterpret_cast<unsigned short *>(c.v_mid_4 + at / 2) = (unsigned short)((w0 & 0xF0) | ((w1 >> 4) & 15) | (w2 & 0xF0) << 8 | ((w3 >> 4) & 15) << 8);
-        *reinterpret_cast<unsigned short *>(c.v_last_4 + at / 2) = (unsigned short)((w0 & 15) << 4 | (w1 & 15) | (w2 & 15) << 12 | (w3 & 15) << 8);
-    } else {
-        // channel-major rows: 64 tokens of a channel are 64 + 32 + 32 bytes; a thread writes 4 tokens
-        const int d = threadIdx.x >> 4, r = (threadIdx.x & 15) * 4;
-        const u32 w0 = tile[r][d], w1 = tile[r + 1][d], w2 = tile[r + 2][d], w3 = tile[r + 3][d];
-        const int64_t at = ((bh * c.n_max_blocks + flushed / c.k_block) * D + ch0 + d) * c.k_block + flushed % c.k_block + r;
-        *reinterpret_cast<u32 *>(c.k_first_8 + at) = (w0 >> 8) | (w1 & 0xFF00u) | (w2 & 0xFF00u) << 8 | (w3 & 0xFF00u) << 16;
-        *reinterpret_cast<unsigned short *>(c.k_mid_4 + at / 2) = (unsigned short)((w0 & 0xF0) | ((w1 >> 4) & 15) | (w2 & 0xF0) << 8 | ((w3 >> 4) & 15) << 8);
-        *reinterpret_cast<unsigned short *>(c.k_last_4 + at / 2) = (unsigned short)((w0 & 15) << 4 | (w1 & 15) | (w2 & 15) << 12 | (w3 & 15) << 8);
+    // four elements side by side in a plane at a time: four channels of a token (values), four tokens of a channel (keys)
+    for (int id = tid; id < kRest * D / 4; id += 256) {
+        const int r = is_v ? id / LANES : id % (kRest / 4) * 4, d = is_v ? id % LANES * 4 : id / (kRest / 4), next = is_v ? 1 : PITCH;
+        const unsigned short *e = &tile[r * PITCH + d];
+        const u32 w0 = e[0], w1 = e[next], w2 = e[2 * next], w3 = e[3 * next];
+        const int64_t at = is_v ? (bh * c.max_seq_len + flushed + r) * D + d
+                                : ((bh * c.n_max_blocks + flushed / c.k_block) * D + d) * c.k_block + flushed % c.k_block + r;
+        *reinterpret_cast<u32 *>((is_v ? c.v_first_8 : c.k_first_8) + at) = (w0 >> 8) | (w1 & 0xFF00u) | (w2 & 0xFF00u) << 8 | (w3 & 0xFF00u) << 16;
+        *reinterpret_cast<unsigned short *>((is_v ? c.v_mid_4 : c.k_mid_4) + at / 2) =
+            (unsigned short)((w0 & 0xF0) | ((w1 >> 4) & 15) | (w2 & 0xF0) << 8 | ((w3 >> 4) & 15) << 8);
+        *reinterpret_cast<unsigned short *>((is_v ? c.v_last_4 : c.k_last_4) + at / 2) =
+            (unsigned short)((w0 & 15) << 4 | (w1 & 15) | (w2 & 15) << 12 | (w3 & 15) << 8);
     }
 }
 
-// The lengths, once every workgroup of the launch before has read them.
-__global__ __launch_bounds__(64) void tree_commit_lens_kernel(CommitArgs a) {
-    const akv_cache_layer &c = a.c[blockIdx.y];
-    const int b = blockIdx.x;
-    const int x = (int)threadIdx.x < a.A ? a.accepted[b * a.A + threadIdx.x] : -1;
-    const unsigned long long ok = __ballot(x >= 0 && x < a.T);
-    if (threadIdx.x == 0) {
-        const int n = max(0, c.seq_lens[b]);
-        c.seq_lens[b] = n + max(0, min(ok == ~0ull ? 64 : (int)__builtin_ctzll(~ok), c.max_seq_len - n));
-    }
+// The lengths, once every workgroup of the launches before has read them.
+constexpr int kLensLayers = 240;
+struct CommitLens {
+    int *seq_lens[kLensLayers];
+    int capacity[kLensLayers];
+    const int *accepted;
+    int T, A;
+};
+static_assert(sizeof(CommitLens) <= 4096, "kernel arguments");
+__global__ __launch_bounds__(64) void tree_commit_lens_kernel(CommitLens a) {
+    const int b = blockIdx.x, lane = threadIdx.x;
+    const int index = lane < a.A ? a.accepted[b * a.A + lane] : -1;
+    int *lens = a.seq_lens[blockIdx.y];
+    const int n = max(0, lens[b]), count = accepted_count(index, a.T, n, a.capacity[blockIdx.y]);
+    if (lane == 0) lens[b] = n + count;
 }
 
 int check_layer(const akv_cache_layer *c, const char *what) {
@@ -564,24 +581,41 @@ extern "C" int akv_tree_commit(const akv_cache_layer *layers, int n_layers, cons
         const int rc = akv::check_layer(layers + i, "tree_commit");
         if (rc != AKV_OK) return rc;
         AKV_REQUIRE(k[i] && v[i], "tree_commit: null pointer");
+        AKV_REQUIRE((((uintptr_t)k[i] | (uintptr_t)v[i]) & 7) == 0, "tree_commit: k and v must be 8-byte aligned");
         AKV_REQUIRE(layers[i].bsz == layers[0].bsz && layers[i].n_kv_heads == layers[0].n_kv_heads && layers[i].head_dim == layers[0].head_dim,
                     "tree_commit: layer %d has another shape than layer 0", i);
         for (int j = 0; j < i; ++j)
             AKV_REQUIRE(layers[i].seq_lens != layers[j].seq_lens, "tree_commit: layers %d and %d share their lengths", j, i);
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int streams = layers[0].bsz * layers[0].n_kv_heads;
     for (int first = 0; first < n_layers; first += akv::kCommitLayers) {
         const int count = n_layers - first < akv::kCommitLayers ? n_layers - first : akv::kCommitLayers;
         akv::CommitArgs a;
         for (int i = 0; i < count; ++i) {
-            a.c[i] = layers[first + i];
-            a.k[i] = k[first + i];
-            a.v[i] = v[first + i];
+            const akv_cache_layer &c = layers[first + i];
+            a.c[i] = {c.k_first_8, c.k_mid_4, c.k_last_4, c.v_first_8, c.v_mid_4, c.v_last_4, c.k_exp_column_max, c.v_exp_column_max, c.restk, c.restv,
+                      c.seq_lens, k[first + i], v[first + i], c.n_max_blocks, c.max_seq_len, c.k_block};
         }
         a.accepted = accepted;
         a.T = n_drafts;
         a.A = n_accepted;
-        hipLaunchKernelGGL(akv::tree_commit_kernel, dim3(layers[0].head_dim / 16 * 2, layers[0].bsz * layers[0].n_kv_heads, count), dim3(256), 0, st, a);
+        a.H = layers[0].n_kv_heads;
+        const dim3 grid(2, streams, count);
+        if (layers[0].head_dim == 64) hipLaunchKernelGGL(akv::tree_commit_kernel<64>, grid, dim3(256), 0, st, a);
+        else if (layers[0].head_dim == 128) hipLaunchKernelGGL(akv::tree_commit_kernel<128>, grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(akv::tree_commit_kernel<256>, grid, dim3(256), 0, st, a);
+    }
+    for (int first = 0; first < n_layers; first += akv::kLensLayers) {
+        const int count = n_layers - first < akv::kLensLayers ? n_layers - first : akv::kLensLayers;
+        akv::CommitLens a;
+        for (int i = 0; i < count; ++i) {
+            a.seq_lens[i] = layers[first + i].seq_lens;
+            a.capacity[i] = layers[first + i].max_seq_len;
+        }
+        a.accepted = accepted;
+        a.T = n_drafts;
+        a.A = n_accepted;
         hipLaunchKernelGGL(akv::tree_commit_lens_kernel, dim3(layers[0].bsz, count), dim3(64), 0, st, a);
     }
     return akv::check_launch("tree_commit");

@@ -17,7 +17,11 @@ rest_tokens = 64
 
 
 def _tensor(name, t, dtype, shape, device=None, contiguous=True):
-    """Checks one argument; shape entries of None are free."""
+    """Checks one argument; shape entries of None are free.  (A call is a few microseconds of host time altogether: the common case is
+    told in one expression, what is wrong with an argument is worked out only where something is.)"""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.shape == shape and (device is None or t.device == device) \
+            and (not contiguous or t.is_contiguous()):
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
     if t.dtype != dtype:
@@ -32,6 +36,27 @@ def _tensor(name, t, dtype, shape, device=None, contiguous=True):
     if contiguous and not t.is_contiguous():
         raise RuntimeError(f"{name}: must be contiguous")
     return t
+
+
+def _dims(name, t, n):
+    """The shape of an argument of n dimensions."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    s = t.shape
+    if len(s) != n:
+        raise RuntimeError(f"{name}: expected {n} dimensions, got shape {list(s)}")
+    return s
+
+
+def _call(fn, device, *args):
+    """One library call on `device`, its current stream last; raises what the library reports."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream_ptr(device))
+    if rc != 0:
+        check(rc)
 
 
 def _number(name, x, low, strict):
@@ -52,50 +77,38 @@ def _strided(name, t):
     return t, s
 
 
-class _Prompt:
-    """An akv_prompt_desc and the tensors behind it."""
-
-    def __init__(self, q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents):
-        _tensor("q", q, torch.half, (None, None, None, None), contiguous=False)
-        B, S, Hq, D = q.shape
-        dev = q.device
-        _tensor("k", k, torch.half, (B, S, None, D), dev, contiguous=False)
-        Hkv = k.shape[2]
-        if v is not None:
-            _tensor("v", v, torch.half, (B, S, Hkv, D), dev, contiguous=False)
-        if D not in (64, 128, 256):
-            raise RuntimeError(f"head_dim {D}: 64, 128 or 256")
-        if B < 1 or S < 1 or Hkv < 1 or Hq < 1 or Hq % Hkv:
-            raise RuntimeError(f"q {list(q.shape)} and k {list(k.shape)}: at least one sequence and token, query heads a multiple of the KV heads")
-        scale = 1.0 / math.sqrt(D) if scale is None else _number("scale", scale, 0.0, True)
-        softcap = _number("softcap", softcap, 0.0, False)
-        if slopes is not None:
-            _tensor("slopes", slopes, torch.float32, (Hq,), dev)
-        if seq_lens is not None:
-            _tensor("seq_lens", seq_lens, torch.int32, (B,), dev)
-        if prefix_lens is not None:
-            _tensor("prefix_lens", prefix_lens, torch.int32, (B,), dev)
-        if documents is not None:
-            _tensor("documents", documents, torch.int32, (B, S), dev)
-        self.shape = (B, S, Hq, Hkv, D)
-        self.device = dev
-        d = self.desc = PromptDesc()
-        self.keep = []
-        for name, t in (("q", q), ("k", k), ("v", v)):
-            if t is None:
-                continue
-            t, s = _strided(name, t)
-            self.keep.append(t)
-            setattr(d, name, t.data_ptr())
-            getattr(d, name + "_stride")[:] = s[:3]
-        d.slopes, d.seq_lens, d.prefix_lens, d.documents = _ptr(slopes), _ptr(seq_lens), _ptr(prefix_lens), _ptr(documents)
-        d.bsz, d.seqlen, d.n_q_heads, d.n_kv_heads, d.head_dim = B, S, Hq, Hkv, D
-        d.scale, d.softcap = scale, softcap
-
-
-def _on(device):
-    """The device made current for a launch (nothing to do when it is)."""
-    return torch.cuda.device(device)
+def _prompt(q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents):
+    """An akv_prompt_desc, what it describes (B, S, Hq, Hkv, D), the device, and the tensors behind it."""
+    B, S, Hq, D = shape = _dims("q", q, 4)
+    dev = q.device
+    _tensor("q", q, torch.half, shape, contiguous=False)
+    Hkv = _dims("k", k, 4)[2]
+    _tensor("k", k, torch.half, (B, S, Hkv, D), dev, contiguous=False)
+    if v is not None:
+        _tensor("v", v, torch.half, (B, S, Hkv, D), dev, contiguous=False)
+    if D not in (64, 128, 256):
+        raise RuntimeError(f"head_dim {D}: 64, 128 or 256")
+    if B < 1 or S < 1 or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise RuntimeError(f"q {list(q.shape)} and k {list(k.shape)}: at least one sequence and token, query heads a multiple of the KV heads")
+    scale = D ** -0.5 if scale is None else _number("scale", scale, 0.0, True)
+    softcap = _number("softcap", softcap, 0.0, False) if softcap else 0.0
+    if slopes is not None:
+        _tensor("slopes", slopes, torch.float32, (Hq,), dev)
+    if seq_lens is not None:
+        _tensor("seq_lens", seq_lens, torch.int32, (B,), dev)
+    if prefix_lens is not None:
+        _tensor("prefix_lens", prefix_lens, torch.int32, (B,), dev)
+    if documents is not None:
+        _tensor("documents", documents, torch.int32, (B, S), dev)
+    q, qs = _strided("q", q)
+    k, ks = _strided("k", k)
+    vp, vs = None, ks
+    if v is not None:
+        v, vs = _strided("v", v)
+        vp = v.data_ptr()
+    desc = PromptDesc(q.data_ptr(), k.data_ptr(), vp, *qs[:3], *ks[:3], *vs[:3], _ptr(slopes), _ptr(seq_lens), _ptr(prefix_lens), _ptr(documents),
+                      B, S, Hq, Hkv, D, scale, softcap)
+    return desc, (B, S, Hq, Hkv, D), dev, (q, k, v)
 
 
 def prefill_attention(self, q, k, v, *, scale=None, softcap=0.0, slopes=None, seq_lens=None, prefix_lens=None, documents=None, out=None,
@@ -107,24 +120,22 @@ def prefill_attention(self, q, k, v, *, scale=None, softcap=0.0, slopes=None, se
     they were); prefix_lens int32 [B]: the first tokens are seen by every row; documents int32 [B, S]: rows see tokens of their own
     document only (several prompts packed in one row; a negative id sees nothing and is not seen)."""
     lib = load_library()
-    p = _Prompt(q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents)
     if v is None:
         raise TypeError("v: expected a torch.Tensor, got NoneType")
-    B, S, Hq, _, D = p.shape
+    desc, (B, S, Hq, _, D), dev, _held = _prompt(q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents)
     fill = out is None
     if fill:
-        out = torch.empty((B, S, Hq, D), dtype=torch.half, device=p.device)
+        out = torch.empty((B, S, Hq, D), dtype=torch.half, device=dev)
     else:
-        _tensor("out", out, torch.half, (B, S, Hq, D), p.device)
-    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=p.device) if return_lse else None
+        _tensor("out", out, torch.half, (B, S, Hq, D), dev)
+    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=dev) if return_lse else None
     if lse is not None and not fill and seq_lens is not None:
         lse.fill_(-math.inf)
     ws, need = None, 0
     if documents is not None:
         need = lib.akv_prefill_attention_workspace_bytes(B, S)
-        ws = torch.empty(need, dtype=torch.uint8, device=p.device)
-    with _on(p.device):
-        check(lib.akv_prefill_attention(ctypes.byref(p.desc), out.data_ptr(), _ptr(lse), 1 if fill else 0, _ptr(ws), need, _stream_ptr(p.device)), lib)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(lib.akv_prefill_attention, dev, ctypes.byref(desc), out.data_ptr(), _ptr(lse), 1 if fill else 0, _ptr(ws), need)
     return (out, lse) if return_lse else out
 
 
@@ -134,27 +145,28 @@ def attention_weights(self, q, k, lse, *, scale=None, softcap=0.0, slopes=None, 
     `window` rows of each sequence (0: all rows).  lse: what prefill_attention returned for the same q, k, masks and score form.
     out: fp32 [B, Hkv, >= S] (dense last dimension) to add the weights to instead; it is returned."""
     lib = load_library()
-    p = _Prompt(q, k, None, scale, softcap, slopes, seq_lens, prefix_lens, documents)
-    B, S, Hq, Hkv, D = p.shape
-    _tensor("lse", lse, torch.float32, (B, Hq, S), p.device)
+    desc, (B, S, Hq, Hkv, D), dev, _held = _prompt(q, k, None, scale, softcap, slopes, seq_lens, prefix_lens, documents)
+    _tensor("lse", lse, torch.float32, (B, Hq, S), dev)
     window = int(window)
     if window < 0:
         raise RuntimeError(f"window: {window} must be 0 (every row) or positive")
     add = out is not None
     if not add:
-        out = torch.empty((B, Hkv, S), dtype=torch.float32, device=p.device)
+        out = torch.empty((B, Hkv, S), dtype=torch.float32, device=dev)
     else:
-        _weights("out", out, B, Hkv, S, p.device)
-    with _on(p.device):
-        check(lib.akv_attention_weights(ctypes.byref(p.desc), lse.data_ptr(), min(window, 1 << 30), out.data_ptr(), out.stride(0), out.stride(1), 1 if add else 0,
-                                        _stream_ptr(p.device)), lib)
+        _weights("out", out, B, Hkv, S, dev)
+    _call(lib.akv_attention_weights, dev, ctypes.byref(desc), lse.data_ptr(), min(window, 1 << 30), out.data_ptr(), out.stride(0), out.stride(1),
+          1 if add else 0)
     return out
 
 
 def _weights(name, t, B, H, n, device):
     """An accumulator: fp32 [B, H, >= n], rows dense and apart."""
-    _tensor(name, t, torch.float32, (B, H, None), device, contiguous=False)
-    if t.shape[2] < n:
+    have = _dims(name, t, 3)[2]
+    _tensor(name, t, torch.float32, (B, H, have), device, contiguous=False)
+    if have >= n and t.is_contiguous():
+        return t
+    if have < n:
         raise RuntimeError(f"{name}: rows of {t.shape[2]} weights for {n} tokens")
     if t.stride(2) != 1 or (H > 1 and t.stride(1) < t.shape[2]) or (B > 1 and t.stride(0) < (t.stride(1) if H > 1 else t.shape[2])):
         raise RuntimeError(f"{name}: rows must be dense and must not overlap")
@@ -167,11 +179,10 @@ def accumulate_weights(self, weights, probs, seq_lens, *, decay=1.0, out=None):
     fp16 [B, Hq, width], the record of the fused step (width a multiple of 8, at least the capacity); seq_lens int32 [B] after the step.
     out: where the sums go (default: weights itself); it is returned."""
     lib = load_library()
-    _tensor("probs", probs, torch.half, (None, None, None))
-    B, Hq, width = probs.shape
+    B, Hq, width = shape = _dims("probs", probs, 3)
     dev = probs.device
-    _tensor("weights", weights, torch.float32, (B, None, None), dev, contiguous=False)
-    Hkv, cap = weights.shape[1], weights.shape[2]
+    _tensor("probs", probs, torch.half, shape)
+    _, Hkv, cap = _dims("weights", weights, 3)
     _weights("weights", weights, B, Hkv, cap, dev)
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise RuntimeError(f"probs {list(probs.shape)}, weights {list(weights.shape)}: query heads must be a multiple of the KV heads")
@@ -185,9 +196,8 @@ def accumulate_weights(self, weights, probs, seq_lens, *, decay=1.0, out=None):
         out = weights
     else:
         _weights("out", out, B, Hkv, cap, dev)
-    with _on(dev):
-        check(lib.akv_accumulate_weights(weights.data_ptr(), weights.stride(0), weights.stride(1), probs.data_ptr(), width, seq_lens.data_ptr(), out.data_ptr(),
-                                         out.stride(0), out.stride(1), B, Hq, Hkv, cap, decay, _stream_ptr(dev)), lib)
+    _call(lib.akv_accumulate_weights, dev, weights.data_ptr(), weights.stride(0), weights.stride(1), probs.data_ptr(), width, seq_lens.data_ptr(),
+          out.data_ptr(), out.stride(0), out.stride(1), B, Hq, Hkv, cap, decay)
     return out
 
 
@@ -198,6 +208,9 @@ class PreparedLayer:
     def __init__(self, desc, device, keep):
         self.desc = desc
         self.device = device
+        self.kind = (device, desc.bsz, desc.n_kv_heads, desc.head_dim)
+        self.lens = desc.seq_lens
+        self.pointers = tuple(t.data_ptr() for t in keep)
         self._keep = keep
 
     @property
@@ -244,7 +257,7 @@ def _layer(self, layer):
     return layer if isinstance(layer, PreparedLayer) else self.prepare_layer(*layer)
 
 
-def _aligned(name, t):
+def _aligned(t):
     if not t.is_contiguous():
         t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -261,8 +274,8 @@ def tree_attention(self, layer, q, k, v, ancestors=None, *, scale=None, softcap=
     layer = _layer(self, layer)
     c, dev = layer.desc, layer.device
     B, H, D = c.bsz, c.n_kv_heads, c.head_dim
-    _tensor("q", q, torch.half, (B, None, None, D), dev, contiguous=False)
-    T, Hq = q.shape[1], q.shape[2]
+    _, T, Hq, _ = _dims("q", q, 4)
+    _tensor("q", q, torch.half, (B, T, Hq, D), dev, contiguous=False)
     if not 1 <= T <= 64:
         raise RuntimeError(f"{T} drafted tokens: 1 to 64")
     if Hq < 1 or Hq % H:
@@ -273,23 +286,22 @@ def tree_attention(self, layer, q, k, v, ancestors=None, *, scale=None, softcap=
         ancestors = chain_ancestors(T, dev)
     else:
         _tensor("ancestors", ancestors, torch.int64, (T,) if ancestors.dim() == 1 else (B, T), dev)
-    scale = 1.0 / math.sqrt(D) if scale is None else _number("scale", scale, 0.0, True)
-    softcap = _number("softcap", softcap, 0.0, False)
+    scale = D ** -0.5 if scale is None else _number("scale", scale, 0.0, True)
+    softcap = _number("softcap", softcap, 0.0, False) if softcap else 0.0
     if slopes is not None:
         _tensor("slopes", slopes, torch.float32, (Hq,), dev)
     bound = c.max_seq_len if bound is None else int(bound)
     if not 0 <= bound <= c.max_seq_len:
         raise RuntimeError(f"bound: {bound} outside [0, {c.max_seq_len}]")
-    q, k, v = _aligned("q", q), _aligned("k", k), _aligned("v", v)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
     if out is None:
         out = torch.empty((B, T, Hq, D), dtype=torch.half, device=dev)
     else:
         _tensor("out", out, torch.half, (B, T, Hq, D), dev)
     need = lib.akv_tree_attention_workspace_bytes(B, Hq, H, D, T, bound)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        check(lib.akv_tree_attention(ctypes.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), ancestors.data_ptr(), 1 if ancestors.dim() == 2 else 0,
-                                     _ptr(slopes), scale, softcap, out.data_ptr(), T, Hq, bound, ws.data_ptr(), need, _stream_ptr(dev)), lib)
+    _call(lib.akv_tree_attention, dev, ctypes.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), ancestors.data_ptr(),
+          1 if ancestors.dim() == 2 else 0, _ptr(slopes), scale, softcap, out.data_ptr(), T, Hq, bound, ws.data_ptr(), need)
     return out
 
 
@@ -299,28 +311,28 @@ def tree_commit(self, layers, k, v, accepted):
     (A at most 64): the accepted drafts of each sequence in order, ended by any entry outside [0, T), -1 say.  Tokens beyond the
     capacity are dropped."""
     lib = load_library()
-    layers = [_layer(self, x) for x in layers]
+    layers = [x if type(x) is PreparedLayer else self.prepare_layer(*x) for x in layers]
     if not layers:
         raise RuntimeError("layers: at least one")
     N, c, dev = len(layers), layers[0].desc, layers[0].device
-    shape = (c.bsz, None, c.n_kv_heads, c.head_dim)
+    shape, kind = (c.bsz, None, c.n_kv_heads, c.head_dim), layers[0].kind
     for i, x in enumerate(layers):
-        if x.device != dev or (x.desc.bsz, x.desc.n_kv_heads, x.desc.head_dim) != (c.bsz, c.n_kv_heads, c.head_dim):
+        if x.kind != kind:
             raise RuntimeError(f"layers: layer {i} has another shape or device than layer 0")
-    if len({x.desc.seq_lens for x in layers}) != N:
+    if len({x.lens for x in layers}) != N:
         raise RuntimeError("layers: the same layer (or the same lengths) twice")
     pointers, keep, T = [], [], None
     for name, t in (("k", k), ("v", v)):
         if isinstance(t, torch.Tensor):
-            _tensor(name, t, torch.half, (N, *shape), dev, contiguous=False)
-            t = _aligned(name, t)
+            _tensor(name, t, torch.half, (N, c.bsz, _dims(name, t, 5)[2], c.n_kv_heads, c.head_dim), dev, contiguous=False)
+            t = _aligned(t)
             keep.append(t)
             step = t.stride(0) * 2
             ps, here = [t.data_ptr() + i * step for i in range(N)], t.shape[2]
         else:
             if len(t) != N:
                 raise RuntimeError(f"{name}: {len(t)} tensors for {N} layers")
-            t = [_aligned(name, _tensor(name, x, torch.half, shape, dev, contiguous=False)) for x in t]
+            t = [_aligned(_tensor(name, x, torch.half, shape, dev, contiguous=False)) for x in t]
             keep.append(t)
             ps, here = [x.data_ptr() for x in t], t[0].shape[1]
             if any(x.shape[1] != here for x in t):
@@ -331,12 +343,11 @@ def tree_commit(self, layers, k, v, accepted):
         pointers.append((ctypes.c_void_p * N)(*ps))
     if not 1 <= T <= 64:
         raise RuntimeError(f"{T} drafted tokens: 1 to 64")
-    _tensor("accepted", accepted, torch.int32, (c.bsz, None), dev)
+    _tensor("accepted", accepted, torch.int32, (c.bsz, _dims("accepted", accepted, 2)[1]), dev)
     if not 1 <= accepted.shape[1] <= 64:
         raise RuntimeError(f"accepted: {accepted.shape[1]} entries a sequence: 1 to 64")
     descs = (CacheLayer * N)(*(x.desc for x in layers))
-    with _on(dev):
-        check(lib.akv_tree_commit(descs, N, pointers[0], pointers[1], accepted.data_ptr(), T, accepted.shape[1], _stream_ptr(dev)), lib)
+    _call(lib.akv_tree_commit, dev, descs, N, pointers[0], pointers[1], accepted.data_ptr(), T, accepted.shape[1])
 
 
 def evict(self, layer, weights, keep, *, sinks=0, recent=0, into=None, into_weights=None):
@@ -351,11 +362,10 @@ def evict(self, layer, weights, keep, *, sinks=0, recent=0, into=None, into_weig
     src = _layer(self, layer)
     dst = src if into is None else _layer(self, into)
     c, d, dev = src.desc, dst.desc, src.device
-    if dst.device != dev or (c.bsz, c.n_kv_heads, c.head_dim, c.k_block) != (d.bsz, d.n_kv_heads, d.head_dim, d.k_block):
+    if src.kind != dst.kind or c.k_block != d.k_block:
         raise RuntimeError("into: must have the batch, heads, head_dim, k_block and device of the cache")
-    same = [getattr(c, f) == getattr(d, f) for f, _ in CacheLayer._fields_[:11]]
-    in_place = all(same)
-    if any(same) and not in_place:
+    in_place = src.pointers == dst.pointers
+    if not in_place and any(x == y for x, y in zip(src.pointers, dst.pointers)):
         raise RuntimeError("into: shares some of its tensors with the cache")
     keep, sinks, recent = int(keep), int(sinks), int(recent)
     if keep < 64 or keep % 64:
@@ -379,10 +389,9 @@ def evict(self, layer, weights, keep, *, sinks=0, recent=0, into=None, into_weig
     kept = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
     need = lib.akv_evict_workspace_bytes(B, H, c.head_dim, c.k_block, keep, 1 if in_place else 0)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        check(lib.akv_evict(ctypes.byref(c), ctypes.byref(d), weights.data_ptr(), weights.stride(0), weights.stride(1), _ptr(to),
-                            to.stride(0) if to is not None else 0, to.stride(1) if to is not None else 0, to.shape[2] if to is not None else 0, kept.data_ptr(),
-                            keep, sinks, recent, ws.data_ptr(), need, _stream_ptr(dev)), lib)
+    ts = (to.data_ptr(), to.stride(0), to.stride(1), to.shape[2]) if to is not None else (None, 0, 0, 0)
+    _call(lib.akv_evict, dev, ctypes.byref(c), ctypes.byref(d), weights.data_ptr(), weights.stride(0), weights.stride(1), *ts, kept.data_ptr(), keep, sinks,
+          recent, ws.data_ptr(), need)
     return kept
 
 

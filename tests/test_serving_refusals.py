@@ -33,12 +33,13 @@ def mem():
 def prompt(mem, **kw):
     d = _lib.PromptDesc()
     d.q = d.k = d.v = mem
-    for n in ("q_stride", "k_stride", "v_stride"):
-        getattr(d, n)[:] = (64 * 4 * 16, 64 * 4, 64)
+    for n in "qkv":
+        kw.setdefault(n + "_stride", (64 * 4 * 16, 64 * 4, 64))
     d.bsz, d.seqlen, d.n_q_heads, d.n_kv_heads, d.head_dim, d.scale, d.softcap = 1, 16, 4, 4, 64, 0.125, 0.0
     for n, x in kw.items():
         if n.endswith("_stride"):
-            getattr(d, n)[:] = x
+            for i, s in zip("bsh", x):
+                setattr(d, f"{n}_{i}", s)
         else:
             setattr(d, n, x)
     return d
