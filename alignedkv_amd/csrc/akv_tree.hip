@@ -382,20 +382,22 @@ __device__ __forceinline__ int accepted_count(int index, int T, int n, int capac
     return max(0, min(ok == ~0ull ? 64 : (int)__builtin_ctzll(~ok), capacity - n));
 }
 
-// grid (2, B * Hkv, layers), 256 threads: the keys (blockIdx.x 0) or the values of one KV head.
+// grid (2 * D / 64, B * Hkv, layers), 256 threads: 64 channels of the keys (even blockIdx.x) or the values of one KV head: the tile
+// then takes 17 KB of LDS and eight workgroups share a compute unit.
 template <int D>
 __global__ __launch_bounds__(256) void tree_commit_kernel(CommitArgs a) {
     const CommitLayer &c = a.c[blockIdx.z];
-    constexpr int PITCH = D + 2, LANES = D / 4;          // a row of the tile in halves; threads to a row, four channels each
+    constexpr int CH = 64, PITCH = CH + 2, LANES = CH / 4;          // a row of the tile in halves; threads to a row, four channels each
     __shared__ __attribute__((aligned(16))) unsigned short tile[2 * kRest * PITCH];
-    const bool is_v = blockIdx.x;
+    const bool is_v = blockIdx.x & 1;
+    const int ch0 = (blockIdx.x >> 1) * CH;
     const int H = a.H, b = blockIdx.y / H, h = blockIdx.y - b * H, tid = threadIdx.x, lane = tid & 63;
     const int index = lane < a.A ? a.accepted[b * a.A + lane] : -1;
     const int n = max(0, c.seq_lens[b]), n_rest = n % kRest, flushed = n - n_rest;
     const int count = accepted_count(index, a.T, n, c.max_seq_len);
     if (count == 0) return;
-    unsigned short *rest = reinterpret_cast<unsigned short *>(is_v ? c.restv : c.restk) + ((int64_t)b * kRest * H + h) * D;
-    const unsigned short *draft = reinterpret_cast<const unsigned short *>(is_v ? c.v : c.k) + ((int64_t)b * a.T * H + h) * D;
+    unsigned short *rest = reinterpret_cast<unsigned short *>(is_v ? c.restv : c.restk) + ((int64_t)b * kRest * H + h) * D + ch0;
+    const unsigned short *draft = reinterpret_cast<const unsigned short *>(is_v ? c.v : c.k) + ((int64_t)b * a.T * H + h) * D + ch0;
     const int64_t row = (int64_t)H * D;
     const int total = n_rest + count;
     const bool flush = total >= kRest;
@@ -412,8 +414,8 @@ __global__ __launch_bounds__(256) void tree_commit_kernel(CommitArgs a) {
         }
     }
     __syncthreads();
-    uint8_t *colmax = (is_v ? c.v_max : c.k_max) + ((int64_t)b * H + h) * D;
-    if (tid < D) {
+    uint8_t *colmax = (is_v ? c.v_max : c.k_max) + ((int64_t)b * H + h) * D + ch0;
+    if (tid < CH) {
         int mx = colmax[tid];
         for (int r = n_rest; r < total; ++r) mx = max(mx, (tile[r * PITCH + tid] >> 10) & 31);
         colmax[tid] = (uint8_t)mx;
@@ -429,12 +431,12 @@ __global__ __launch_bounds__(256) void tree_commit_kernel(CommitArgs a) {
     if (!flush) return;
     const int64_t bh = (int64_t)b * H + h;
     // four elements side by side in a plane at a time: four channels of a token (values), four tokens of a channel (keys)
-    for (int id = tid; id < kRest * D / 4; id += 256) {
+    for (int id = tid; id < kRest * CH / 4; id += 256) {
         const int r = is_v ? id / LANES : id % (kRest / 4) * 4, d = is_v ? id % LANES * 4 : id / (kRest / 4), next = is_v ? 1 : PITCH;
         const unsigned short *e = &tile[r * PITCH + d];
         const u32 w0 = e[0], w1 = e[next], w2 = e[2 * next], w3 = e[3 * next];
-        const int64_t at = is_v ? (bh * c.max_seq_len + flushed + r) * D + d
-                                : ((bh * c.n_max_blocks + flushed / c.k_block) * D + d) * c.k_block + flushed % c.k_block + r;
+        const int64_t at = is_v ? (bh * c.max_seq_len + flushed + r) * D + ch0 + d
+                                : ((bh * c.n_max_blocks + flushed / c.k_block) * D + ch0 + d) * c.k_block + flushed % c.k_block + r;
         *reinterpret_cast<u32 *>((is_v ? c.v_first_8 : c.k_first_8) + at) = (w0 >> 8) | (w1 & 0xFF00u) | (w2 & 0xFF00u) << 8 | (w3 & 0xFF00u) << 16;
         *reinterpret_cast<unsigned short *>((is_v ? c.v_mid_4 : c.k_mid_4) + at / 2) =
             (unsigned short)((w0 & 0xF0) | ((w1 >> 4) & 15) | (w2 & 0xF0) << 8 | ((w3 >> 4) & 15) << 8);
@@ -601,7 +603,7 @@ extern "C" int akv_tree_commit(const akv_cache_layer *layers, int n_layers, cons
         a.T = n_drafts;
         a.A = n_accepted;
         a.H = layers[0].n_kv_heads;
-        const dim3 grid(2, streams, count);
+        const dim3 grid(2 * layers[0].head_dim / 64, streams, count);
         if (layers[0].head_dim == 64) hipLaunchKernelGGL(akv::tree_commit_kernel<64>, grid, dim3(256), 0, st, a);
         else if (layers[0].head_dim == 128) hipLaunchKernelGGL(akv::tree_commit_kernel<128>, grid, dim3(256), 0, st, a);
         else hipLaunchKernelGGL(akv::tree_commit_kernel<256>, grid, dim3(256), 0, st, a);
