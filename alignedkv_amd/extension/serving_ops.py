@@ -66,6 +66,18 @@ def _number(name, x, low, strict):
     return x
 
 
+def _apart(name, out, *inputs):
+    """Refuses an `out` that shares memory with an input: workgroups write theirs while others still read."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    lo, hi = span(out)
+    for t in inputs:
+        if t is not None and t.numel():
+            a, b = span(t)
+            if a < hi and lo < b:
+                raise RuntimeError(f"{name}: overlaps an input")
+
+
 def _strided(name, t):
     """(pointer, strides) of a [batch, tokens, heads, head_dim] fp16 view, or of a contiguous copy where the kernels cannot read the view."""
     s = t.stride()
@@ -118,7 +130,8 @@ def prefill_attention(self, q, k, v, *, scale=None, softcap=0.0, slopes=None, se
     score(i, j) = cap(scale q_i . k_j) - slopes[h] |i - j|, cap(x) = softcap tanh(x / softcap) (softcap 0: x); scale: 1 / sqrt(D).
     seq_lens int32 [B]: tokens at and beyond a length are padding (rows of zeros, lse -inf; with `out` given these rows are left as
     they were); prefix_lens int32 [B]: the first tokens are seen by every row; documents int32 [B, S]: rows see tokens of their own
-    document only (several prompts packed in one row; a negative id sees nothing and is not seen)."""
+    document only (several prompts packed in one row; a negative id sees nothing and is not seen).
+    No gradient is recorded, as by every operator here."""
     lib = load_library()
     if v is None:
         raise TypeError("v: expected a torch.Tensor, got NoneType")
@@ -128,6 +141,7 @@ def prefill_attention(self, q, k, v, *, scale=None, softcap=0.0, slopes=None, se
         out = torch.empty((B, S, Hq, D), dtype=torch.half, device=dev)
     else:
         _tensor("out", out, torch.half, (B, S, Hq, D), dev)
+        _apart("out", out, q, k, v)
     lse = torch.empty((B, Hq, S), dtype=torch.float32, device=dev) if return_lse else None
     if lse is not None and not fill and seq_lens is not None:
         lse.fill_(-math.inf)
@@ -196,6 +210,8 @@ def accumulate_weights(self, weights, probs, seq_lens, *, decay=1.0, out=None):
         out = weights
     else:
         _weights("out", out, B, Hkv, cap, dev)
+        if out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride():
+            _apart("out", out, weights)
     _call(lib.akv_accumulate_weights, dev, weights.data_ptr(), weights.stride(0), weights.stride(1), probs.data_ptr(), width, seq_lens.data_ptr(),
           out.data_ptr(), out.stride(0), out.stride(1), B, Hq, Hkv, cap, decay)
     return out
@@ -212,6 +228,10 @@ class PreparedLayer:
         self.lens = desc.seq_lens
         self.pointers = tuple(t.data_ptr() for t in keep)
         self._keep = keep
+
+    def made_of(self, tensors) -> bool:
+        """Whether these are the tensors it was made of."""
+        return all(x is y for x, y in zip(self._keep, tensors))
 
     @property
     def seq_lens(self):
@@ -298,6 +318,7 @@ def tree_attention(self, layer, q, k, v, ancestors=None, *, scale=None, softcap=
         out = torch.empty((B, T, Hq, D), dtype=torch.half, device=dev)
     else:
         _tensor("out", out, torch.half, (B, T, Hq, D), dev)
+        _apart("out", out, q, k, v)
     need = lib.akv_tree_attention_workspace_bytes(B, Hq, H, D, T, bound)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(lib.akv_tree_attention, dev, ctypes.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), ancestors.data_ptr(),

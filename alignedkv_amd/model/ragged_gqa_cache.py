@@ -132,9 +132,10 @@ class RaggedGQACache:
 
     # ---- whole prompts, drafted tokens, eviction ---------------------------------------------------------------------
     def prepared(self, layer: int):
-        """The layer's descriptor for cuda_module.tree_attention / tree_commit / evict, made once (its tensors stay for the
-        cache's life)."""
-        if self._prepared[layer] is None:
+        """The layer's descriptor for cuda_module.tree_attention / tree_commit / evict, made once for these tensors."""
+        now = (*self.k_planes[layer], *self.v_planes[layer], self.k_colmax[layer], self.v_colmax[layer], self.restk[layer],
+               self.restv[layer], self.seq_lens[layer])
+        if self._prepared[layer] is None or not self._prepared[layer].made_of(now):
             self._prepared[layer] = cuda_module.prepare_layer(
                 self.k_planes[layer], self.v_planes[layer], self.k_colmax[layer], self.v_colmax[layer], self.restk[layer],
                 self.restv[layer], self.seq_lens[layer])

@@ -209,3 +209,32 @@ def test_a_cache_without_weights_refuses_to_evict():
     c._evicted[0][0] = True
     with pytest.raises(RuntimeError, match="positions"):
         c.verify(0, None, None, None, slopes=torch.ones(2))
+
+
+def test_an_output_that_overlaps_an_input_is_refused():
+    pool = torch.zeros(4, 8, 16)
+    serving_ops._apart("out", pool[0], pool[1], None, pool[2:])
+    serving_ops._apart("out", pool[1], pool[:0])
+    for out, other in ((pool[0], pool[0]), (pool[1], pool.flatten()[120:160]), (pool[:, 0], pool[2]), (pool[3], pool.expand(2, 4, 8, 16))):
+        with pytest.raises(RuntimeError, match="out: overlaps an input"):
+            serving_ops._apart("out", out, torch.zeros(3), other)
+
+
+def test_a_prepared_layer_follows_the_tensors_of_its_cache():
+    made = []
+    from alignedkv_amd.model.ragged_gqa_cache import RaggedGQACache
+    cache = RaggedGQACache(1, 2, 128, 2, 2, 64, device="cpu")
+    class Module:                                            # noqa: E306
+        @staticmethod
+        def prepare_layer(*a):
+            made.append(serving_ops.PreparedLayer(_lib.CacheLayer(), None, (*a[0], *a[1], *a[2:])))
+            return made[-1]
+    import alignedkv_amd.model.ragged_gqa_cache as module
+    real, module.cuda_module = module.cuda_module, Module
+    try:
+        first = cache.prepared(0)
+        assert cache.prepared(0) is first
+        cache.seq_lens[0] = cache.seq_lens[0] + 1            # a caller's own tensor in the place of the cache's
+        assert cache.prepared(0) is not first and cache.prepared(0).seq_lens is cache.seq_lens[0] and len(made) == 2
+    finally:
+        module.cuda_module = real
