@@ -76,14 +76,16 @@ __device__ __forceinline__ Choice make_choice(int n, int keep, int sinks, int re
 // 11.5 us against 14.8).  The `need`-th largest key is found by its digits, 11 + 11 + 10 bits, each from a
 // histogram in LDS; then the chosen tokens are written in order.  Token THREADS i + thread is this thread's i-th: the keys of the first
 // kHeld * THREADS tokens are read once and kept in registers (32000 tokens: 46 us with every pass reading them, latency, not
-// bytes), those of a longer row again in every pass.
+// bytes, 34 with the registers), those of a longer row again in every pass.  Weights crowd in few exponents: eight histograms side by side,
+// a lane's by its number, keep lanes of one bin apart (32000 tokens 34.5 -> 31.6 us); with 256 threads clearing and adding them costs more than
+// it saves (1000 tokens 11.4 -> 17.3 us), and one does.  Latency bounds it: 8 MB of weights at 8 x 8 rows of 32000.
 constexpr int kHeld = 32;
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void evict_select_kernel(const float *__restrict__ weights, int64_t w_b, int64_t w_h, const int *__restrict__ lens,
                                                             int *__restrict__ kept, int *__restrict__ old_lens, int Hkv, int capacity, int keep, int sinks,
                                                             int recent) {
-    __shared__ u32 hist[2048];
-    constexpr int WAVES = THREADS / 64, BINS = 2048 / THREADS;
+    constexpr int WAVES = THREADS / 64, BINS = 2048 / THREADS, COPIES = THREADS == 1024 ? 8 : 1;
+    __shared__ __attribute__((aligned(16))) u32 hist[2048 * COPIES];
     __shared__ int wave_tot[WAVES];
     __shared__ u32 digit_s;
     __shared__ int above_s;
@@ -118,10 +120,10 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(const float *__re
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < 2048; i += THREADS) hist[i] = 0;
+        for (int i = tid; i < 2048 * COPIES / 4; i += THREADS) reinterpret_cast<u32x4 *>(hist)[i] = u32x4{0u, 0u, 0u, 0u};
         __syncthreads();
         each([&](int j, u32 k) {
-            if (candidate(j) && (pass == 0 || (k >> (shift + bits)) == prefix)) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+            if (candidate(j) && (pass == 0 || (k >> (shift + bits)) == prefix)) atomicAdd(&hist[((k >> shift) & ((1u << bits) - 1)) * COPIES + (lane & (COPIES - 1))], 1u);
         });
         __syncthreads();
         // thread i holds BINS bins below 2048 - BINS i: counts from the top
@@ -129,7 +131,9 @@ __global__ __launch_bounds__(THREADS) void evict_select_kernel(const float *__re
         int own[BINS], inc = 0;
 #pragma unroll
         for (int k = 0; k < BINS; ++k) {
-            own[k] = (int)hist[top - k];
+            own[k] = 0;
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) own[k] += (int)hist[(top - k) * COPIES + i];
             inc += own[k];
         }
         const int mine = inc;
