@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     constexpr int UNITS = D * TT / 16 / 256;         // Raw16 of each side per thread and round
     constexpr int kPart = D * BN * 2;
     constexpr int kBox = 64 * (D / 2 + 2 + D / 32);  // words a wave hands over when the parts are joined
-    constexpr int kLds = 2 * PARTS * kPart > (PARTS - 1) * WAVES * kBox * 4 ? 2 * PARTS * kPart : (PARTS - 1) * WAVES * kBox * 4;
+    constexpr int kBuffers = PARTS == 1 ? 2 : 1, kBuffer = 2 * PARTS * kPart;
+    constexpr int kLds = kBuffers * kBuffer > (PARTS - 1) * WAVES * kBox * 4 ? kBuffers * kBuffer : (PARTS - 1) * WAVES * kBox * 4;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     __shared__ int tail_pos[128];                    // positions of the tail's tokens
     __shared__ int odd_tile[PARTS];
@@ -171,6 +172,50 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     RowState st;
     OddValues<D> odd;
 
+    if constexpr (kBuffers == 2) {
+        // the next round's keys and values go into the other buffer while this one's are multiplied: one barrier a round
+        if (first < end) {
+            put(k_lds, kChStep * BN * 2, kr);
+            put(v_lds, kTokStep * D * 2, vr);
+            if (first + TT < end) {
+                request_k(first + TT);
+                request_v(first + TT);
+            }
+        }
+        lds_barrier();
+        int buf = 0;
+        for (int j0 = first; j0 < end; j0 += TT) {
+            at.pin();
+            asm volatile("" : "+v"(k_at0), "+v"(k_at1), "+v"(k_lds), "+v"(v_lds), "+v"(v_off));
+            const int next = j0 + TT, other = buf ^ kBuffer;
+            f32x16 x[TB];
+            f16x8 p[TB][2];
+            key_scores<D, BN>(x, kt + buf, k_at0, k_at1, qf);
+            if (next < end) {
+                put(k_lds + other, kChStep * BN * 2, kr);
+                if (next + TT < end) request_k(next + TT);
+            }
+            const float factor = modify_block<CAP, TB>(x, a.form);
+            float shift = 0.f;
+            if constexpr (ALIBI) {
+                // every cached token lies before the row: the distance is linear in the token
+                const float s = neg_slope * __builtin_amdgcn_rcpf(factor);       // (the same in every lane; times factor again: 1 ulp of the bias)
+                shift = -neg_slope * (float)(j0 + 4 * half - pos);
+#pragma unroll
+                for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[tb][r] = fmaf(-s, (float)(tb * 32 + 8 * (r >> 2) + place(r & 3)), x[tb][r]);
+            }
+            tile_softmax<D, BN>(x, factor, shift, st, o, p);
+            if (next < end) {
+                put(v_lds + other, kTokStep * D * 2, vr);
+                if (next + TT < end) request_v(next + TT);
+            }
+            tile_output<D, BN>(o, vt + buf, at, p);
+            lds_barrier();
+            buf = other;
+        }
+    } else
     for (int j0 = first; j0 < end; j0 += TT) {
         at.pin();
         asm volatile("" : "+v"(k_at0), "+v"(k_at1), "+v"(k_lds), "+v"(v_lds), "+v"(v_off));
