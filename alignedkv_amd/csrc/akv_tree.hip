@@ -85,10 +85,10 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
 // unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
 // 128 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
 // tree_combine_kernel.
-template <int D, int KB, int PARTS, int BN, bool CAP, bool ALIBI>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
-    constexpr int TT = PARTS * BN, ROWS = 128 / PARTS, WAVES = 4 / PARTS, TB = BN / 32;
-    constexpr int UNITS = D * TT / 16 / 256;         // Raw16 of each side per thread and round
+template <int D, int KB, int PARTS, int BN, int THREADS, bool CAP, bool ALIBI>
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
+    constexpr int TT = PARTS * BN, ROWS = THREADS / 2 / PARTS, WAVES = THREADS / 64 / PARTS, TB = BN / 32;
+    constexpr int UNITS = D * TT / 16 / THREADS;         // Raw16 of each side per thread and round
     constexpr int kPart = D * BN * 2;
     constexpr int kBox = 64 * (D / 2 + 2 + D / 32);  // words a wave hands over when the parts are joined
     constexpr int kBuffers = PARTS == 1 ? 2 : 1, kBuffer = 2 * PARTS * kPart;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
     const int first = split * a.tokens_per_split, end = split < a.plane_splits ? min(first + a.tokens_per_split, flushed) : 0;
     Raw16 kr[UNITS], vr[UNITS];
     // Piece u of a thread lies a constant behind piece 0, in memory and in LDS: four addresses stay in registers.
-    constexpr int kChStep = 256 * 16 / TT, kTokStep = 256 * 16 / D;      // channels / tokens from piece to piece
+    constexpr int kChStep = THREADS * 16 / TT, kTokStep = THREADS * 16 / D;      // channels / tokens from piece to piece
     static_assert(kChStep % 16 == 0 && kTokStep % 16 == 0, "rows 16 apart are laid out alike");
     const int k_tok = tid % (TT / 16) * 16, k_ch = tid / (TT / 16), v_c16 = tid % (D / 16), v_tok = tid / (D / 16);
     int k_lds = k_tok / BN * kPart + key_byte<BN>(k_ch, k_tok % BN / 8);                                // the other half: ^ 16
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a)
         for (int u0 = 0; u0 < total; u0 += TT) {
             lds_barrier();
 #pragma unroll 2
-            for (int id = tid; id < TT * CPR; id += 256) {
+            for (int id = tid; id < TT * CPR; id += THREADS) {
                 const int u = id / CPR, ch = id % CPR, uu = u0 + u;
                 u32x4 kw = {0u, 0u, 0u, 0u}, vw = {0u, 0u, 0u, 0u};
                 if (uu < total) {
@@ -523,21 +523,25 @@ int check_layer(const akv_cache_layer *c, const char *what) {
     return AKV_OK;
 }
 
-// How a call is cut up: the rows of a KV head into groups of 32, 64 or 128 (4, 2 or 1 parts), the planes into splits of whole rounds.
+// How a call is cut up: the rows of a KV head into groups of 32, 64, 128 or 256 (4, 2, 1 or 1 parts), the planes into splits of whole rounds.
 struct TreePlan {
-    int parts, tokens, groups, plane_splits, tokens_per_split, splits;
+    int parts, row_tile, tokens, groups, plane_splits, tokens_per_split, splits;
 };
 static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int bound) {
     TreePlan p;
     p.parts = rows > 64 ? 1 : (rows > 32 ? 2 : 4);
     p.tokens = p.parts == 4 ? 128 : p.parts * (head_dim == 256 ? 32 : 64);
-    p.groups = (rows + 128 / p.parts - 1) / (128 / p.parts);
+    // 512 threads share a round's planes, loaded and unpacked once, where there are the rows for them: 4 x 16384 tokens x 8 KV heads, 256 rows
+    // 118 us against 125 with 256 threads, 264 to 512 rows 178 to 185 against 196 to 199; 136 rows 134 against 130.  (head_dim 256: the
+    // registers of a wave, two to a SIMD, do not hold it; 64: too few planes a round to share.)
+    p.row_tile = head_dim == 128 && rows > 128 ? 256 : 128 / p.parts;
+    p.groups = (rows + p.row_tile - 1) / p.row_tile;
     const int flushed = bound / kRest * kRest, rounds = (flushed + p.tokens - 1) / p.tokens;
     const int64_t units = (int64_t)bsz * n_kv_heads * p.groups;
     // Workgroups in one round of the chip: two a compute unit (one with head_dim 256, which takes the registers of both).  Where the
     // planes' traffic, not the arithmetic, is what a call waits for, fewer of them leave fewer sums to join: 16 drafts x 4 heads a KV head
     // over 8 x 8150 tokens 50.3 us with 384 against 56.6 with 512; 64 drafts over 4 x 32768, which is arithmetic, 297 against 258.
-    const int aim = head_dim == 256 ? 256 : (p.parts == 1 ? 512 : 384);
+    const int aim = head_dim == 256 ? 256 : (p.row_tile == 256 ? 256 : p.parts == 1 ? 512 : 384);
     int64_t want = (aim + units - 1) / units;
     if (want > rounds) want = rounds;
     if (want < 1) want = 1;
@@ -553,15 +557,16 @@ static void launch_tree(const TreeArgs &a, const TreePlan &p, bool cap, hipStrea
     const dim3 grid((u32)(((int64_t)p.splits * a.c.n_kv_heads * a.c.bsz + 7) / 8 * 8 * p.groups));
     const bool alibi = a.slopes != nullptr;
     constexpr int BN = D == 256 ? 32 : 64;
-#define AKV_TREE(PARTS, BN, CAP, ALIBI) hipLaunchKernelGGL((tree_kernel<D, KB, PARTS, BN, CAP, ALIBI>), grid, dim3(256), 0, st, a)
-#define AKV_TREE_PARTS(PARTS, BN)                                                                                         \
+#define AKV_TREE(PARTS, BN, THREADS, CAP, ALIBI) hipLaunchKernelGGL((tree_kernel<D, KB, PARTS, BN, THREADS, CAP, ALIBI>), grid, dim3(THREADS), 0, st, a)
+#define AKV_TREE_PARTS(PARTS, BN, THREADS)                                                                                         \
     do {                                                                                                                  \
-        if (cap) { if (alibi) AKV_TREE(PARTS, BN, true, true); else AKV_TREE(PARTS, BN, true, false); }                   \
-        else { if (alibi) AKV_TREE(PARTS, BN, false, true); else AKV_TREE(PARTS, BN, false, false); }                     \
+        if (cap) { if (alibi) AKV_TREE(PARTS, BN, THREADS, true, true); else AKV_TREE(PARTS, BN, THREADS, true, false); }                   \
+        else { if (alibi) AKV_TREE(PARTS, BN, THREADS, false, true); else AKV_TREE(PARTS, BN, THREADS, false, false); }                     \
     } while (0)
-    if (p.parts == 4) AKV_TREE_PARTS(4, 32);
-    else if (p.parts == 2) AKV_TREE_PARTS(2, BN);
-    else AKV_TREE_PARTS(1, BN);
+    if (p.parts == 4) AKV_TREE_PARTS(4, 32, 256);
+    else if (p.parts == 2) AKV_TREE_PARTS(2, BN, 256);
+    else if (p.row_tile == 128) AKV_TREE_PARTS(1, BN, 256);
+    else if constexpr (D == 128) AKV_TREE_PARTS(1, BN, 512);
 #undef AKV_TREE_PARTS
 #undef AKV_TREE
     hipLaunchKernelGGL(tree_combine_kernel<D>, dim3((a.rows + 1024 / D - 1) / (1024 / D), a.c.n_kv_heads, a.c.bsz), dim3(256), 0, st, a);
