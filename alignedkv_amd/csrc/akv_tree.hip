@@ -8,6 +8,7 @@
 namespace akv {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 constexpr int kRest = 64;       // tokens of the rest buffer
 
 struct TreeArgs {
@@ -17,14 +18,82 @@ struct TreeArgs {
     int anc_stride;                       // T or 0
     const float *slopes;
     uint8_t *out;
-    float *parts;                         // [B * Hkv, splits, rows] x {D sums}, then the same x {m, l}
+    float *parts;                         // [Hkv, splits, rows] x {D sums}, then the same x {m, l}
+    int *shares;                          // [B] x {first split, splits}
     int T, Hq, G, rows;                   // rows = T * G
-    int plane_splits, tokens_per_split, splits;
+    int log_tokens, splits, own_tail;     // of a round's tokens; of all sequences together, for a KV head; the tail has a split of its own
     ScoreForm form;
 };
 
 // Cached tokens of a sequence, kept inside the planes whatever the device holds.
 __device__ __forceinline__ int cached_tokens(const TreeArgs &a, int b) { return max(0, min(a.c.seq_lens[b], a.c.max_seq_len)); }
+
+// Which stretch of which sequence split u is.  The splits are dealt out by the lengths: every one takes the same number of rounds, the
+// fewest with which all sequences together need no more than there are, so that a ragged batch does not wait for its longest sequence (8
+// sequences of 1000 to 8000 tokens, 8 KV heads x 128, 5 drafts: 47 us against 59 with as many splits for each, 32 of 100 to 9400 131 against 156).
+struct Share {
+    int b, split, count, tokens;      // tokens: of a split of the planes
+};
+// Rounds of a split: an odd number where it is not small, so that splits that run side by side do not start a power of two apart in memory,
+// which crowds them on the same memory channels (8 x 4096 tokens x 32 heads: 116 -> 112 us).
+__device__ __forceinline__ int odd_rounds(int per) { return per >= 8 ? per | 1 : per; }
+// ceil(a / b) for 0 <= a <= 2^24, 0 < b (more rounds than that do not fit the memory; the quotient before it is cut off is then wrong by
+// less than one: 2^-23 and 2^-24 of at most 2^24 / 3, and exact for one and two; an integer division is three times as long, and a workgroup waits for this)
+__device__ __forceinline__ int ceil_div(int a, int b) {
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));       // off by one at most
+    int rest = a - q * b;
+    if (rest < 0) rest += b, --q;
+    return q + (rest > 0 ? 1 : 0) + (rest > b ? 1 : 0);
+}
+__device__ __forceinline__ bool find_share(const TreeArgs &a, int u, Share &s) {
+    const int B = a.c.bsz, lane = threadIdx.x & 63, least = 1 - a.own_tail, planes = a.splits - B * a.own_tail;
+    const auto rounds_of = [&](int b) { return (cached_tokens(a, b) / kRest * kRest + (1 << a.log_tokens) - 1) >> a.log_tokens; };
+    if (B == 1) {
+        const int r = rounds_of(0), per = odd_rounds(max(1, ceil_div(r, planes)));
+        s = {0, u, max(least, ceil_div(r, per)) + a.own_tail, per << a.log_tokens};
+        return u < s.count;
+    }
+    // a lane a sequence, 64 at a time; -1: none
+    const int r0 = lane < B ? rounds_of(lane) : -1;
+    const auto rounds_at = [&](int c) { return c == 0 ? r0 : (c + lane < B ? rounds_of(c + lane) : -1); };
+    const auto splits_of = [&](int r, int per) { return r < 0 ? 0 : max(least, ceil_div(r, per)) + a.own_tail; };
+    int all = 0, longest = 1;
+    for (int c = 0; c < B; c += 64) {
+        const int r = rounds_at(c);
+        all += wave_sum_i32(max(r, 0));
+        longest = max(longest, (int)~wave_min_u32(~(u32)max(r, 0)));
+    }
+    int lo = max(1, (int)((u32)(all + planes - 1) / (u32)planes)), hi = longest;
+    const int spare = planes - B;       // (a sequence needs fewer than r / per + 1 splits of its planes)
+    if (spare > 0) hi = min(hi, max(lo, (int)((u32)(all + spare - 1) / (u32)spare)));
+    int per = lo;
+    while (lo < hi) {
+        int need = 0;
+        for (int c = 0; c < B; c += 64) need += wave_sum_i32(splits_of(rounds_at(c), per));
+        if (need <= a.splits) hi = per;
+        else lo = per + 1;
+        per = (lo + hi) >> 1;
+    }
+    per = odd_rounds(hi);
+    int before = 0;
+    for (int c = 0; c < B; c += 64) {
+        const int n = splits_of(rounds_at(c), per);
+        int inc = n;
+        const int in_chunk = min(B - c, 64);
+        for (int d = 1; d < in_chunk; d <<= 1) {
+            const int o = __shfl_up(inc, d);
+            if (lane >= d) inc += o;
+        }
+        const unsigned long long past = __ballot(u < before + inc);
+        if (past) {
+            const int l = __builtin_ctzll(past), count = __builtin_amdgcn_readlane(n, l);
+            s = {c + l, u - (before + __builtin_amdgcn_readlane(inc, l) - count), count, per << a.log_tokens};
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(inc, in_chunk - 1);
+    }
+    return false;
+}
 
 // 16-bit values of elements 0,2 / 1,3 / 4,6 / 5,7 of 8 elements (high bytes Ha, Hb; nibbles M, L).  They are used in this order: four
 // elements 0 1 2 3 lie at places 0 2 1 3, which costs nothing where the order of tokens or channels is free.
@@ -80,8 +149,8 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
     }
 }
 
-// grid: a workgroup per split, row group, KV head and sequence (see unit below); 256 threads.  Split s < plane_splits: tiles of the planes; the last split: the rest buffer and the
-// drafts (behind its share of the planes, if it has one).  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
+// grid: a workgroup per split, row group and KV head (see unit below).  A sequence's splits: stretches of the planes; the last one: the rest buffer and the
+// drafts, behind its stretch unless the tail has a split of its own.  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
 // unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
 // 128 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
 // tree_combine_kernel.
@@ -101,16 +170,19 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
     // Workgroups are dealt out to the 8 XCDs in turn: the row groups of a stretch of the planes are 8 apart, so that one XCD's L2 serves
     // them all.
     const int unit = (int)(blockIdx.x / 8 / groups) * 8 + (int)(blockIdx.x % 8), rg = blockIdx.x / 8 % groups;
-    if (unit >= a.splits * a.c.n_kv_heads * a.c.bsz) return;
-    const int split = unit % a.splits, hkv = unit / a.splits % a.c.n_kv_heads, b = unit / a.splits / a.c.n_kv_heads;
+    const int hkv = unit / a.splits, slot = unit - hkv * a.splits;
+    Share share;
+    if (hkv >= a.c.n_kv_heads || !find_share(a, slot, share)) return;
+    const int b = share.b, split = share.split;
+    if (hkv == 0 && rg == 0 && split == 0 && tid == 0) *reinterpret_cast<i32x2 *>(a.shares + 2 * b) = i32x2{slot, share.count};
     const int n = cached_tokens(a, b), flushed = n / kRest * kRest, n_rest = n - flushed, total = n_rest + a.T;
     const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv;
     const int row = rg * ROWS + (wave % WAVES) * 32 + (lane & 31), row_c = min(row, a.rows - 1), g = row_c / a.T, t = row_c - g * a.T;
-    const bool tail = split == a.splits - 1;
+    const bool tail = split == share.count - 1;
     uint8_t *kt = lds + part * kPart, *vt = lds + PARTS * kPart + part * kPart;
 
     // the planes: this thread's pieces of a round
-    const int first = split * a.tokens_per_split, end = split < a.plane_splits ? min(first + a.tokens_per_split, flushed) : 0;
+    const int first = split * share.tokens, end = split < share.count - a.own_tail ? min(first + share.tokens, flushed) : 0;
     Raw16 kr[UNITS], vr[UNITS];
     // Piece u of a thread lies a constant behind piece 0, in memory and in LDS: four addresses stay in registers.
     constexpr int kChStep = THREADS * 16 / TT, kTokStep = THREADS * 16 / D;      // channels / tokens from piece to piece
@@ -354,8 +426,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
         st.m = m;
     }
     if (row >= a.rows) return;
-    float *po = a.parts + ((bh * a.splits + split) * a.rows + row) * D;
-    float *pm = a.parts + (int64_t)a.c.bsz * a.c.n_kv_heads * a.splits * a.rows * D + ((bh * a.splits + split) * a.rows + row) * 2;
+    float *po = a.parts + ((int64_t)unit * a.rows + row) * D;
+    float *pm = a.parts + (int64_t)a.c.n_kv_heads * a.splits * a.rows * D + ((int64_t)unit * a.rows + row) * 2;
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb)
 #pragma unroll
@@ -373,23 +445,25 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
     constexpr int LANES = D / 4, ROWS = 256 / LANES;
     const int row = blockIdx.x * ROWS + threadIdx.x / LANES, hkv = blockIdx.y, b = blockIdx.z, ch = threadIdx.x % LANES * 4;
     if (row >= a.rows) return;
-    const int64_t bh = (int64_t)b * a.c.n_kv_heads + hkv, step = (int64_t)a.rows * D;
-    const float *po = a.parts + bh * a.splits * step + (int64_t)row * D + ch;
-    const f32x2 *pm = reinterpret_cast<const f32x2 *>(a.parts + (int64_t)a.c.bsz * a.c.n_kv_heads * a.splits * step) + bh * a.splits * a.rows + row;
+    const i32x2 share = *reinterpret_cast<const i32x2 *>(a.shares + 2 * b);
+    const int splits = share.y;
+    const int64_t first = (int64_t)hkv * a.splits + share.x, step = (int64_t)a.rows * D;
+    const float *po = a.parts + first * step + (int64_t)row * D + ch;
+    const f32x2 *pm = reinterpret_cast<const f32x2 *>(a.parts + (int64_t)a.c.n_kv_heads * a.splits * step) + first * a.rows + row;
     float m = kNegInf, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+    for (int s0 = 0; s0 < splits; s0 += 4) {
         f32x4 x[4];
         f32x2 ml[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = min(s0 + i, a.splits - 1);
+            const int s = min(s0 + i, splits - 1);
             x[i] = *reinterpret_cast<const f32x4 *>(po + s * step);
             ml[i] = pm[(int64_t)s * a.rows];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (s0 + i >= a.splits) break;
+            if (s0 + i >= splits) break;
             const float top = fmaxf(m, ml[i].x);
             const float f0 = m == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m - top), f1 = ml[i].x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - top);
             o = o * f0 + x[i] * f1;
@@ -525,7 +599,7 @@ int check_layer(const akv_cache_layer *c, const char *what) {
 
 // How a call is cut up: the rows of a KV head into groups of 32, 64, 128 or 256 (4, 2, 1 or 1 parts), the planes into splits of whole rounds.
 struct TreePlan {
-    int parts, row_tile, tokens, groups, plane_splits, tokens_per_split, splits;
+    int parts, row_tile, tokens, groups, splits, own_tail;
 };
 static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int bound) {
     TreePlan p;
@@ -538,23 +612,22 @@ static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int b
     p.groups = (rows + p.row_tile - 1) / p.row_tile;
     const int flushed = bound / kRest * kRest, rounds = (flushed + p.tokens - 1) / p.tokens;
     const int64_t units = (int64_t)bsz * n_kv_heads * p.groups;
-    // Workgroups in one round of the chip: two a compute unit (one with head_dim 256, which takes the registers of both).  Where the
-    // planes' traffic, not the arithmetic, is what a call waits for, fewer of them leave fewer sums to join: 16 drafts x 4 heads a KV head
-    // over 8 x 8150 tokens 50.3 us with 384 against 56.6 with 512; 64 drafts over 4 x 32768, which is arithmetic, 297 against 258.
-    const int aim = head_dim == 256 ? 256 : (p.row_tile == 256 ? 256 : p.parts == 1 ? 512 : 384);
+    // Workgroups in one round of the chip: two a compute unit, one where a workgroup takes the registers of both.  16 drafts x 4 heads a KV
+    // head over 8 sequences of 4075 to 8150 tokens: 58 us with 512, 64 with 384, 66 with 256; of 8192 each 76, 72 and 73 (more sums
+    // to join).  With head_dim 64 the sums weigh more beside the planes: 8 drafts x 4 heads over 4 x 16384 tokens 41 us with 512, 34 with 384.
+    const int aim = head_dim == 256 || p.row_tile == 256 ? 256 : (head_dim == 64 && p.parts > 1 ? 384 : 512);
     int64_t want = (aim + units - 1) / units;
     if (want > rounds) want = rounds;
     if (want < 1) want = 1;
-    p.tokens_per_split = rounds > 0 ? (int)((rounds + want - 1) / want) * p.tokens : p.tokens;
-    p.plane_splits = (flushed + p.tokens_per_split - 1) / p.tokens_per_split;
-    // the tail gets a workgroup of its own while there are compute units without one
-    p.splits = p.plane_splits + (p.plane_splits == 0 || units * (p.plane_splits + 1) <= 256 ? 1 : 0);
+    // the tails get workgroups of their own while there are compute units without one
+    p.own_tail = rounds > 0 && units * (want + 1) <= 256;
+    p.splits = (int)(want + p.own_tail) * bsz;
     return p;
 }
 
 template <int D, int KB>
 static void launch_tree(const TreeArgs &a, const TreePlan &p, bool cap, hipStream_t st) {
-    const dim3 grid((u32)(((int64_t)p.splits * a.c.n_kv_heads * a.c.bsz + 7) / 8 * 8 * p.groups));
+    const dim3 grid((u32)(((int64_t)p.splits * a.c.n_kv_heads + 7) / 8 * 8 * p.groups));
     const bool alibi = a.slopes != nullptr;
     constexpr int BN = D == 256 ? 32 : 64;
 #define AKV_TREE(PARTS, BN, THREADS, CAP, ALIBI) hipLaunchKernelGGL((tree_kernel<D, KB, PARTS, BN, THREADS, CAP, ALIBI>), grid, dim3(THREADS), 0, st, a)
@@ -578,7 +651,7 @@ extern "C" size_t akv_tree_attention_workspace_bytes(int bsz, int n_q_heads, int
     if (bsz < 1 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || head_dim < 1 || n_drafts < 1 || n_drafts > 64 || len_bound < 0) return 0;
     const int rows = n_q_heads / n_kv_heads * n_drafts;
     const akv::TreePlan p = akv::tree_plan(bsz, n_kv_heads, head_dim, rows, len_bound);
-    return (size_t)bsz * n_kv_heads * p.splits * rows * (head_dim + 2) * sizeof(float);
+    return (size_t)n_kv_heads * p.splits * rows * (head_dim + 2) * sizeof(float) + (size_t)bsz * 2 * sizeof(int);
 }
 
 extern "C" int akv_tree_attention(const akv_cache_layer *layer, const uint8_t *q, const uint8_t *k, const uint8_t *v, const int64_t *ancestors,
@@ -607,8 +680,9 @@ extern "C" int akv_tree_attention(const akv_cache_layer *layer, const uint8_t *q
     a.T = n_drafts; a.Hq = n_q_heads; a.G = n_q_heads / layer->n_kv_heads; a.rows = a.T * a.G;
     a.form = akv::score_form(scale, softcap);
     const akv::TreePlan p = akv::tree_plan(layer->bsz, layer->n_kv_heads, layer->head_dim, a.rows, len_bound);
-    a.plane_splits = p.plane_splits; a.tokens_per_split = p.tokens_per_split; a.splits = p.splits;
-    AKV_REQUIRE(((int64_t)p.splits * layer->n_kv_heads * layer->bsz + 8) * p.groups < (1ll << 31), "tree_attention: too many rows");
+    a.log_tokens = __builtin_ctz((unsigned)p.tokens); a.splits = p.splits; a.own_tail = p.own_tail;
+    a.shares = reinterpret_cast<int *>(a.parts + (size_t)layer->n_kv_heads * p.splits * a.rows * (layer->head_dim + 2));
+    AKV_REQUIRE(((int64_t)p.splits * layer->n_kv_heads + 8) * p.groups < (1ll << 31), "tree_attention: too many rows");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool cap = softcap > 0.f;
     if (layer->k_block == 64) {
