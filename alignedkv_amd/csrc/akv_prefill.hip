@@ -130,6 +130,11 @@ __device__ __forceinline__ void prompt_block(int id, int n_tiles, int B, int Hkv
     hq = (stream - b * Hkv) * G + rest % G;
 }
 
+// One pass over the tokens with a running maximum and sum in 32 bits (the sum is rescaled only when the maximum has grown by 2^8); scores are
+// computed transposed, so that a lane owns a query row and its probabilities are the second product's operand where they are, rounded
+// to fp16 for it (2^-11 of each; its sums are in 32 bits).  Bound by the arithmetic: 8192 tokens, 32 heads over 8 x 128, causal, 816 to 963 TFLOP/s
+// of the 1251 that a large fp16 matrix product reaches here; head_dim 64 800, where a score's scaling and exponential weigh twice as much beside its
+// products; head_dim 256 600, a wave to a SIMD.
 // grid n_tiles * Hq * B, 256 threads.  K and V tiles of BN tokens go through LDS, two buffers, filled by asynchronous loads: the
 // next tiles are in flight while these are computed, one barrier a round.  PARTS == 1: 128 query rows of one head, 32 a wave, all
 // on the same tile.  PARTS == 2: 64 rows, two waves on every other tile each, their sums joined at the end: half the rounds for a
@@ -365,7 +370,8 @@ __global__ __launch_bounds__(256, D == 256 || D * PARTS == 256 ? 1 : (D == 64 &&
 // w_j = sum over the heads g of the group and the rows i of the window of exp(s_ij - lse_i).  A workgroup owns 128 tokens of one KV
 // head, a wave 32 of them, whose keys stay in registers; the rows, head after head, stream past them through LDS, QR at a
 // time, two buffers filled by asynchronous loads (rows read by their lanes straight from memory, 32 lines a request, kept the address
-// units busy: 39 us at 2 x 8000 tokens, 64 rows of 32 heads).  A lane sums its row's column of each product, and one
+// units busy: 39 us at 2 x 8000 tokens, 64 rows of 32 heads over 8 x 128, 17 through LDS).  Its bound: 33 MB of keys (6.5 us) and, behind them
+// because all workgroups start with their keys, 8.4 GFLOP with an exponential a score.  A lane sums its row's column of each product, and one
 // reduction over the rows' lanes ends it.  No atomics: the order of a sum is fixed.
 template <int D, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256) void attention_weights_kernel(PromptArgs a, const float *__restrict__ lse, int window, float *__restrict__ w,

@@ -149,10 +149,15 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
     }
 }
 
+// o_t = sum_j softmax_j(cap(scale q_t . k_j) - slope (pos_t - pos_j)) v_j over the cache and the drafts that t sees, one pass with a running
+// maximum and sum in 32 bits; probabilities go to fp16 for the second product (2^-11 of each; its sums are in 32 bits).
+// Bound by the planes' bytes while a KV head has few rows (one draft, 8 x 4096 tokens x 32 heads x 128: 112 us, 4.8 TB/s), by what the
+// vector units do for a score beside the products -- unpacking, scaling, one exponential -- where it has many (64 drafts x 4 heads a KV head over
+// 4 x 32768: 205 us, 669 TFLOP/s).
 // grid: a workgroup per split, row group and KV head (see unit below).  A sequence's splits: stretches of the planes; the last one: the rest buffer and the
 // drafts, behind its stretch unless the tail has a split of its own.  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
 // unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
-// 128 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
+// THREADS / 2 / PARTS rows a workgroup, so few rows do not leave waves idle.  The parts' sums are joined through LDS, the splits' by
 // tree_combine_kernel.
 template <int D, int KB, int PARTS, int BN, int THREADS, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArgs a) {
@@ -245,7 +250,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
     OddValues<D> odd;
 
     if constexpr (kBuffers == 2) {
-        // the next round's keys and values go into the other buffer while this one's are multiplied: one barrier a round
+        // the next round's keys and values go into the other buffer while this one's are multiplied: one barrier a round (64 drafts x 4 heads
+        // over 4 x 32768: 234 us against 257 with one buffer and two barriers; with more parts two buffers do not leave room for a second
+        // workgroup)
         if (first < end) {
             put(k_lds, kChStep * BN * 2, kr);
             put(v_lds, kTokStep * D * 2, vr);
@@ -439,7 +446,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
     }
 }
 
-// Joins the splits of a row in order: D / 4 lanes a row, four channels a lane, four splits' sums requested at a time.
+// Joins the splits of a row in order: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 4 lanes a row, four channels a lane, four splits'
+// sums requested at a time: latency and the sums' bytes (4 to 5 us behind a call's 11 to 50).  Joined in the order of the splits, so that the
+// bits do not depend on which workgroup ends first.
 template <int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
     constexpr int LANES = D / 4, ROWS = 256 / LANES;
@@ -480,7 +489,8 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
 // accepted[b]: indices of drafts, in order, up to the first one that is not in [0, T).  They are appended as decode steps would:
 // rest rows, a flush of 64 tokens into the planes when the rest buffer fills (at most one: 63 + 64 < 128), column maxima, lengths.
 // What bounds it is latency: lengths, then indices, then rows, each a round trip, and few bytes behind them.  All layers of a
-// model go into one launch, their descriptors as kernel arguments.
+// model go into one launch, their descriptors as kernel arguments: 24 layers x 8 sequences x 8 heads x 128, 16 drafts: 15 us and 2 for the
+// lengths (a launch a layer: 79 us).
 constexpr int kCommitLayers = 30;      // (4 KB of arguments)
 struct CommitLayer {
     uint8_t *k_first_8, *k_mid_4, *k_last_4, *v_first_8, *v_mid_4, *v_last_4, *k_max, *v_max, *restk, *restv;
