@@ -210,10 +210,10 @@ def accumulate_weights(self, weights, probs, seq_lens, *, decay=1.0, out=None):
         out = weights
     else:
         _weights("out", out, B, Hkv, cap, dev)
-        if out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride():
-            _apart("out", out, weights)
-    _call(lib.akv_accumulate_weights, dev, weights.data_ptr(), weights.stride(0), weights.stride(1), probs.data_ptr(), width, seq_lens.data_ptr(),
-          out.data_ptr(), out.stride(0), out.stride(1), B, Hq, Hkv, cap, decay)
+    (wb, wh, _), (ob, oh, _), w, o = weights.stride(), out.stride(), weights.data_ptr(), out.data_ptr()
+    if (w != o or wb != ob or wh != oh) and w < o + 4 * ((B - 1) * ob + (Hkv - 1) * oh + cap) and o < w + 4 * ((B - 1) * wb + (Hkv - 1) * wh + cap):
+        raise RuntimeError("out: overlaps an input")
+    _call(lib.akv_accumulate_weights, dev, w, wb, wh, probs.data_ptr(), width, seq_lens.data_ptr(), o, ob, oh, B, Hq, Hkv, cap, decay)
     return out
 
 

@@ -135,3 +135,15 @@ def test_large_rows():
     kept = cuda_module.evict(cache.prepared(0), cache.weights[0], 6400)[0, 0]
     order = w.sort(dim=0, descending=True, stable=True).indices[:6400].sort().values
     assert torch.equal(kept.long(), order)
+
+
+def test_sums_into_rows_that_overlap_the_weights_are_refused():
+    from alignedkv_amd.extension.KV_cache_cpp_extention import cuda_module
+    pool = torch.zeros(3, 2, 2, 64, device="cuda")
+    probs, lens = torch.zeros(2, 4, 64, device="cuda", dtype=torch.half), torch.full((2,), 64, dtype=torch.int32, device="cuda")
+    flat = pool.flatten()
+    for out in (flat[64:64 + 256].view(2, 2, 64), flat[4:260].view(2, 2, 64), pool[:, 0].permute(1, 0, 2)[:, :2]):
+        with pytest.raises(RuntimeError, match="out: "):
+            cuda_module.accumulate_weights(pool[0], probs, lens, out=out)
+    for out in (pool[0], pool[1], flat[256:512].view(2, 2, 64)):
+        assert cuda_module.accumulate_weights(pool[0], probs, lens, out=out) is out
