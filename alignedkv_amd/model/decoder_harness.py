@@ -183,7 +183,8 @@ class DeviceLengthCache:
 
     def snapshot(self):
         c = self.inner
-        return [(c.seq_lens[i].clone(), c.k_colmax[i].clone(), c.v_colmax[i].clone()) for i in range(c.n_layers)], list(self._host_len)
+        return [(c.seq_lens[i].clone(), c.k_colmax[i].clone(), c.v_colmax[i].clone()) for i in range(c.n_layers)], list(self._host_len), \
+            None if c.weights is None else [w.clone() for w in c.weights]
 
     def restore(self, snap):
         """Takes back the steps since snapshot(), as long as none of them crossed a 64-token boundary (the token rows
@@ -193,6 +194,8 @@ class DeviceLengthCache:
             c.seq_lens[i].copy_(n)
             c.k_colmax[i].copy_(kc)
             c.v_colmax[i].copy_(vc)
+        for w, was in zip(c.weights or (), snap[2] or ()):
+            w.copy_(was)
         self._host_len = list(snap[1])
 
 

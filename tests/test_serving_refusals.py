@@ -238,3 +238,14 @@ def test_a_prepared_layer_follows_the_tensors_of_its_cache():
         assert cache.prepared(0) is not first and cache.prepared(0).seq_lens is cache.seq_lens[0] and len(made) == 2
     finally:
         module.cuda_module = real
+
+
+def test_a_step_that_is_taken_back_leaves_no_weights():
+    from alignedkv_amd.model.decoder_harness import DecoderConfig, DeviceLengthCache
+    cache = DeviceLengthCache(DecoderConfig(2, 128, 2, 2, 128, 50), 2, 128, device="cpu", track_weights=True)
+    cache.inner.weights[1][0, 1, 3] = 2.0
+    snap = cache.snapshot()
+    cache.inner.weights[1].add_(1.0)
+    cache.inner.seq_lens[0].add_(1)
+    cache.restore(snap)
+    assert cache.inner.weights[1].sum() == 2.0 and (cache.inner.seq_lens[0] == 0).all()
