@@ -80,8 +80,8 @@ def _apart(name, out, *inputs):
 
 def _strided(name, t):
     """(pointer, strides) of a [batch, tokens, heads, head_dim] fp16 view, or of a contiguous copy where the kernels cannot read the view."""
-    s = t.stride()
-    if s[3] != 1 or any(x % 8 or x < 0 for x in s[:3]) or s[1] >= 1 << 24 or t.data_ptr() % 16:
+    a, b, c, d = s = t.stride()
+    if d != 1 or (a | b | c) & 7 or b >= 1 << 24 or t.data_ptr() & 15:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -227,6 +227,7 @@ class PreparedLayer:
         self.kind = (device, desc.bsz, desc.n_kv_heads, desc.head_dim)
         self.lens = desc.seq_lens
         self.pointers = tuple(t.data_ptr() for t in keep)
+        self.places = frozenset(self.pointers)
         self._keep = keep
 
     def made_of(self, tensors) -> bool:
@@ -386,7 +387,7 @@ def evict(self, layer, weights, keep, *, sinks=0, recent=0, into=None, into_weig
     if src.kind != dst.kind or c.k_block != d.k_block:
         raise RuntimeError("into: must have the batch, heads, head_dim, k_block and device of the cache")
     in_place = src.pointers == dst.pointers
-    if not in_place and any(x == y for x, y in zip(src.pointers, dst.pointers)):
+    if not in_place and not src.places.isdisjoint(dst.places):
         raise RuntimeError("into: shares some of its tensors with the cache")
     keep, sinks, recent = int(keep), int(sinks), int(recent)
     if keep < 64 or keep % 64:
