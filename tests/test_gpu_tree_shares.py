@@ -21,7 +21,7 @@ def test_ragged_batches(lens, T, Hq, Hkv, D, kb):
         check_tree(cache.verify(0, q, k, v, anc, bound=bound), cache, q, k, v, anc)
 
 
-@pytest.mark.parametrize("B", [64, 65, 200])
+@pytest.mark.parametrize("B", [64, 65, 200, 300, 600])
 def test_more_sequences_than_lanes(B):
     lens = [(37 * b) % 400 if b % 7 else 0 for b in range(B)]
     lens[-1] = 1300
