@@ -126,11 +126,12 @@ __device__ __forceinline__ int tile_byte(int row, int chunk) {
 }
 
 // 16 bytes a lane from memory straight into LDS, lane l's at lds_base + 16 l (lds_base: the same in all lanes); nothing passes
-// through registers.  The compiler does not see these loads: wait_tile() before what they bring is read.
+// through registers.  The compiler does not see these loads: wait_tile() before what they bring is read.  M0 holds the LDS address, and
+// one wait state has to lie between its write and the load; inside inline assembly the compiler does not put it there.
 __device__ __forceinline__ u32 lds_address(const void *p) { return (u32)(uintptr_t)(__attribute__((address_space(3))) const void *)p; }
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, u32 lds_base, int byte_off) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds_base)), "v"(byte_off), "s"(r)
-                 : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds_base)), "v"(byte_off), "s"(r)
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // All of this wave's loads have arrived and its LDS reads are done, and so are the other waves'.
