@@ -240,7 +240,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) qf[ks] = *reinterpret_cast<const f16x8 *>(qp + (2 * ks + half) * 16);
     const unsigned long long *anc = a.anc + (int64_t)b * a.anc_stride;
-    const unsigned long long my_anc = anc[t];
+    const unsigned long long named = ~0ull >> (64 - a.T);       // bits at and beyond T name no draft
+    const unsigned long long my_anc = anc[t] & named;
     const int pos = n + __popcll(my_anc & ~(1ull << t));
     const float neg_slope = ALIBI ? a.slopes[hkv * a.G + g] * -kLog2e : 0.f;
     LaneBytes<D> at;
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
         // the rest buffer and the drafts: fp16 rows, keys and values token-major in LDS
         const int H = a.c.n_kv_heads;
         const int64_t row_bytes = (int64_t)H * D * 2, r0 = ((int64_t)b * kRest * H + hkv) * (D * 2), d0 = ((int64_t)b * a.T * H + hkv) * (D * 2);
-        if (tid < total) tail_pos[tid] = tid < n_rest ? flushed + tid : n + __popcll(anc[tid - n_rest] & ~(1ull << (tid - n_rest)));
+        if (tid < total) tail_pos[tid] = tid < n_rest ? flushed + tid : n + __popcll(anc[tid - n_rest] & named & ~(1ull << (tid - n_rest)));
         if (tid < PARTS) odd_tile[tid] = -1;
         constexpr int CPR = D / 8;
         for (int u0 = 0; u0 < total; u0 += TT) {

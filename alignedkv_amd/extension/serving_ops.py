@@ -289,7 +289,8 @@ def tree_attention(self, layer, q, k, v, ancestors=None, *, scale=None, softcap=
     [B, T, Hq, D], k, v fp16 [B, T, Hkv, D]; returns fp16 [B, T, Hq, D].  Every plane is read (no fetch decisions); the cache is not
     changed.  layer: a PreparedLayer, or the seven arguments of prepare_layer.
     ancestors int64 [T] or [B, T]: bit u of entry t: draft t sees draft u (its own bit included); default: a chain, each draft sees
-    itself and those before it.  Draft t stands at position length + (other drafts it sees), which is what `slopes` measures distances from.
+    itself and those before it.  Bits at and beyond T are not looked at.  Draft t stands at position length + (other drafts it sees), which
+    is what `slopes` measures distances from.
     bound: upper bound of the lengths that sizes the launch (default: the capacity)."""
     lib = load_library()
     layer = _layer(self, layer)

@@ -286,10 +286,10 @@ typedef struct akv_cache_layer {
 
 /* Attention of n_drafts (1 to 64) drafted tokens per sequence over the whole cache, every plane read, and over the drafts in their
  * masks: bit u of ancestors[t] (int64, [n_drafts], or [bsz, n_drafts] with ancestors_per_sequence) says that draft t sees draft u, itself
- * included if bit t is set.  Draft t stands at position seq_lens[b] + (number of other drafts it sees).  q, out: fp16
- * [bsz, n_drafts, n_q_heads, head_dim]; k, v: fp16 [bsz, n_drafts, n_kv_heads, head_dim].  len_bound: upper bound of the lengths
- * (it sizes the launch: one that is too low costs time, not tokens).  The cache is not changed.  One draft whose mask is its own bit is a decode step without
- * fetch decisions. */
+ * included if bit t is set; bits at and beyond n_drafts are not looked at.  Draft t stands at position seq_lens[b] + (number of other
+ * drafts it sees).  q, out: fp16 [bsz, n_drafts, n_q_heads, head_dim]; k, v: fp16 [bsz, n_drafts, n_kv_heads, head_dim].  len_bound: upper
+ * bound of the lengths (it sizes the launch: one that is too low costs time, not tokens).  The cache is not changed.  One draft whose mask
+ * is its own bit is a decode step without fetch decisions. */
 AKV_API size_t akv_tree_attention_workspace_bytes(int bsz, int n_q_heads, int n_kv_heads, int head_dim, int n_drafts, int len_bound);
 AKV_API int akv_tree_attention(const akv_cache_layer *layer, const uint8_t *q, const uint8_t *k, const uint8_t *v, const int64_t *ancestors,
                                int ancestors_per_sequence, const float *slopes, float scale, float softcap, uint8_t *out, int n_drafts,
