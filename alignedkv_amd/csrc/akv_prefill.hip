@@ -132,7 +132,7 @@ __device__ __forceinline__ void prompt_block(int id, int n_tiles, int B, int Hkv
 
 // One pass over the tokens with a running maximum and sum in 32 bits (the sum is rescaled only when the maximum has grown by 2^8); scores are
 // computed transposed, so that a lane owns a query row and its probabilities are the second product's operand where they are, rounded
-// to fp16 for it (2^-11 of each; its sums are in 32 bits).  Bound by the arithmetic: 8192 tokens, 32 heads over 8 x 128, causal, 816 to 963 TFLOP/s
+// to fp16 for it (2^-11 of each, or 2^-32 of the row's largest; its sums are in 32 bits).  Bound by the arithmetic: 8192 tokens, 32 heads over 8 x 128, causal, 816 to 963 TFLOP/s
 // of the 1251 that a large fp16 matrix product reaches here; head_dim 64 800, where a score's scaling and exponential weigh twice as much beside its
 // products; head_dim 256 600, a wave to a SIMD.
 // grid n_tiles * Hq * B, 256 threads.  K and V tiles of BN tokens go through LDS, two buffers, filled by asynchronous loads: the
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256, D == 256 || D * PARTS == 256 ? 1 : (D == 64 &&
             }
     }
     if (lse != nullptr && half == 0)
-        lse[((int64_t)b * a.Hq + hq) * a.S + i] = i < n ? (l == 0.f ? kNegInf : (st.m + __builtin_amdgcn_logf(l)) * kLn2) : kNegInf;
+        lse[((int64_t)b * a.Hq + hq) * a.S + i] = i < n ? (l == 0.f ? kNegInf : (st.m - kLift + __builtin_amdgcn_logf(l)) * kLn2) : kNegInf;
 }
 
 // ---- the weight each token received -----------------------------------------------------------------------------------------------

@@ -155,7 +155,8 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
 }
 
 // o_t = sum_j softmax_j(cap(scale q_t . k_j) - slope (pos_t - pos_j)) v_j over the cache and the drafts that t sees, one pass with a running
-// maximum and sum in 32 bits; probabilities go to fp16 for the second product (2^-11 of each; its sums are in 32 bits).
+// maximum and sum in 32 bits; probabilities go to fp16 for the second product (2^-11 of each, or 2^-32 of the split's
+// largest; its sums are in 32 bits).
 // Bound by the planes' bytes while a KV head has few rows (one draft, 8 x 4096 tokens x 32 heads x 128: 112 us, 4.8 TB/s), by what the
 // vector units do for a score beside the products -- unpacking, scaling, one exponential -- where it has many (64 drafts x 4 heads a KV head over
 // 4 x 32768: 205 us, 669 TFLOP/s).
