@@ -340,6 +340,14 @@ __device__ __forceinline__ void tile_softmax(f32x16 (&x)[BN / 32], float factor,
     st.l += sum;
 }
 
+// Whether two stretches of memory share a byte (what is written has to lie apart from what other workgroups still read).
+inline bool share_memory(const void *a, int64_t bytes_a, const void *b, int64_t bytes_b) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + (uintptr_t)bytes_b && y < x + (uintptr_t)bytes_a;
+}
+// Bytes from the first to the last of fp32 rows [B, H, n].
+inline int64_t rows_span(int64_t B, int64_t H, int64_t n, int64_t stride_b, int64_t stride_h) { return 4 * ((B - 1) * stride_b + (H - 1) * stride_h + n); }
+
 int check_layer(const akv_cache_layer *c, const char *what);   // of a cache layer's descriptor: AKV_OK or the error
 
 }  // namespace akv

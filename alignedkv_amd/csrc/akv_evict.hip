@@ -403,6 +403,11 @@ extern "C" int akv_accumulate_weights(const float *weights, int64_t weights_stri
     AKV_REQUIRE(row_stride % 8 == 0 && ((uintptr_t)probs & 15) == 0, "accumulate_weights: probabilities need 16-byte aligned rows");
     AKV_REQUIRE(capacity >= 1 && capacity <= row_stride, "accumulate_weights: capacity %d outside [1, row_stride %d]", capacity, row_stride);
     AKV_REQUIRE(decay == decay && decay <= 1e30f && decay >= -1e30f, "accumulate_weights: decay must be finite");
+    const int64_t span = akv::rows_span(bsz, n_kv_heads, capacity, out_stride_b, out_stride_h);
+    const bool same = out == weights && (bsz == 1 || out_stride_b == weights_stride_b) && (n_kv_heads == 1 || out_stride_h == weights_stride_h);
+    AKV_REQUIRE((same || !akv::share_memory(out, span, weights, akv::rows_span(bsz, n_kv_heads, capacity, weights_stride_b, weights_stride_h))) &&
+                    !akv::share_memory(out, span, probs, (int64_t)bsz * n_q_heads * row_stride * 2),
+                "accumulate_weights: out must be the weights themselves or not overlap them, nor the probabilities");
     const dim3 grid((capacity + 2047) / 2048, n_kv_heads, bsz);
     hipLaunchKernelGGL(akv::accumulate_weights_kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), weights, probs, seq_lens, out, n_q_heads / n_kv_heads,
                        n_kv_heads, row_stride, weights_stride_b, weights_stride_h, out_stride_b, out_stride_h, capacity, decay);
@@ -457,6 +462,10 @@ extern "C" int akv_evict(const akv_cache_layer *from, const akv_cache_layer *to,
     const akv::EvictPlan p = akv::evict_plan(from->bsz, from->n_kv_heads, from->head_dim, from->k_block, keep, in_place);
     AKV_REQUIRE(workspace && workspace_bytes >= p.total && ((uintptr_t)workspace & 15) == 0, "evict: needs a 16-byte aligned workspace of %zu bytes, got %zu", p.total,
                 workspace_bytes);
+    AKV_REQUIRE(weights_to == nullptr || in_place ||
+                    !akv::share_memory(weights, akv::rows_span(from->bsz, from->n_kv_heads, from->max_seq_len, weights_stride_b, weights_stride_h), weights_to,
+                                       akv::rows_span(from->bsz, from->n_kv_heads, weights_to_capacity, to_stride_b, to_stride_h)),
+                "evict: the weights that move to another cache must not overlap those they come from");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int streams = from->bsz * from->n_kv_heads;
     akv::MoveArgs a;

@@ -511,6 +511,14 @@ static int prompt_args(PromptArgs &a, const akv_prompt_desc *d, const char *what
     return AKV_OK;
 }
 
+// Whether a stretch of memory shares a byte with q, k or v.
+static bool shares_inputs(const PromptArgs &a, int D, const void *p, int64_t bytes) {
+    const auto with = [&](const uint8_t *x, int64_t b, int64_t s, int64_t h, int heads) {
+        return x != nullptr && share_memory(p, bytes, x, (a.B - 1) * b + (a.S - 1) * s + (heads - 1) * h + D * 2);
+    };
+    return with(a.q, a.q_b, a.q_s, a.q_h, a.Hq) || with(a.k, a.k_b, a.k_s, a.k_h, a.Hkv) || with(a.v, a.v_b, a.v_s, a.v_h, a.Hkv);
+}
+
 // Two parts a row (64 rows a workgroup) pay only while the workgroups of whole rows leave half of the compute units empty:
 // 512 tokens x 32 heads x 128 14.8 us against 16.6, x 16 heads x 256 24.6 against 33.6; with twice the rows 29.8 against 28.1 (fewer
 // workgroups fit a compute unit, and each tile that is loaded serves half the rows).
@@ -551,12 +559,15 @@ extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, 
     AKV_REQUIRE(a.v && out, "prefill_attention: null pointer");
     AKV_REQUIRE(((uintptr_t)out & 15) == 0, "prefill_attention: out must be 16-byte aligned");
     AKV_REQUIRE((int64_t)((a.S + 63) / 64) * a.Hq * a.B < (1ll << 31), "prefill_attention: too many rows");
+    const size_t need = a.docs ? akv_prefill_attention_workspace_bytes(a.B, a.S) : 0;
+    AKV_REQUIRE(!a.docs || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                "prefill_attention: documents need a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
+    const int64_t rows = (int64_t)a.B * a.S * a.Hq, out_bytes = rows * desc->head_dim * 2;
+    AKV_REQUIRE(!akv::shares_inputs(a, desc->head_dim, out, out_bytes) && (lse == nullptr || (!akv::shares_inputs(a, desc->head_dim, lse, rows * 4) &&
+                !akv::share_memory(out, out_bytes, lse, rows * 4))), "prefill_attention: out and lse must not overlap each other, q, k or v");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int parts = akv::prompt_parts(a);
     if (a.docs) {
-        const size_t need = akv_prefill_attention_workspace_bytes(a.B, a.S);
-        AKV_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
-                    "prefill_attention: documents need a 16-byte aligned workspace of %zu bytes, got %zu", need, workspace_bytes);
         const int tile = desc->head_dim == 256 ? 32 : 64, tiles = (a.S + tile - 1) / tile;
         u32x4 *ranges = static_cast<u32x4 *>(workspace);
         int *order = reinterpret_cast<int *>(ranges + (size_t)a.B * tiles);
@@ -585,6 +596,10 @@ extern "C" int akv_attention_weights(const akv_prompt_desc *desc, const float *l
     AKV_REQUIRE(lse && weights, "attention_weights: null pointer");
     AKV_REQUIRE(window >= 0, "attention_weights: window %d must be 0 (every row) or positive", window);
     AKV_REQUIRE(weights_stride_h >= a.S || a.Hkv == 1, "attention_weights: rows of %lld weights for %d tokens", (long long)weights_stride_h, a.S);
+    const int64_t span = akv::rows_span(a.B, a.Hkv, a.S, weights_stride_b, weights_stride_h);
+    a.v = nullptr;      // (not read)
+    AKV_REQUIRE(!akv::shares_inputs(a, desc->head_dim, weights, span) && !akv::share_memory(weights, span, lse, (int64_t)a.B * a.Hq * a.S * 4),
+                "attention_weights: the weights must not overlap q, k or lse");
     const bool cap = desc->softcap > 0.f;
     const dim3 grid((a.S + 127) / 128, a.Hkv, a.B);
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -135,13 +135,13 @@ def prefill_attention(self, q, k, v, *, scale=None, softcap=0.0, slopes=None, se
     lib = load_library()
     if v is None:
         raise TypeError("v: expected a torch.Tensor, got NoneType")
-    desc, (B, S, Hq, _, D), dev, _held = _prompt(q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents)
+    desc, (B, S, Hq, _, D), dev, held = _prompt(q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents)
     fill = out is None
     if fill:
         out = torch.empty((B, S, Hq, D), dtype=torch.half, device=dev)
     else:
         _tensor("out", out, torch.half, (B, S, Hq, D), dev)
-        _apart("out", out, q, k, v)
+        _apart("out", out, *held, slopes, seq_lens, prefix_lens, documents)
     lse = torch.empty((B, Hq, S), dtype=torch.float32, device=dev) if return_lse else None
     if lse is not None and not fill and seq_lens is not None:
         lse.fill_(-math.inf)
@@ -159,7 +159,7 @@ def attention_weights(self, q, k, lse, *, scale=None, softcap=0.0, slopes=None, 
     `window` rows of each sequence (0: all rows).  lse: what prefill_attention returned for the same q, k, masks and score form.
     out: fp32 [B, Hkv, >= S] (dense last dimension) to add the weights to instead; it is returned."""
     lib = load_library()
-    desc, (B, S, Hq, Hkv, D), dev, _held = _prompt(q, k, None, scale, softcap, slopes, seq_lens, prefix_lens, documents)
+    desc, (B, S, Hq, Hkv, D), dev, (q, k, _) = _prompt(q, k, None, scale, softcap, slopes, seq_lens, prefix_lens, documents)
     _tensor("lse", lse, torch.float32, (B, Hq, S), dev)
     window = int(window)
     if window < 0:
@@ -169,6 +169,7 @@ def attention_weights(self, q, k, lse, *, scale=None, softcap=0.0, slopes=None, 
         out = torch.empty((B, Hkv, S), dtype=torch.float32, device=dev)
     else:
         _weights("out", out, B, Hkv, S, dev)
+        _apart("out", out, q, k, lse, slopes, seq_lens, prefix_lens, documents)
     _call(lib.akv_attention_weights, dev, ctypes.byref(desc), lse.data_ptr(), min(window, 1 << 30), out.data_ptr(), out.stride(0), out.stride(1),
           1 if add else 0)
     return out
@@ -210,8 +211,10 @@ def accumulate_weights(self, weights, probs, seq_lens, *, decay=1.0, out=None):
         out = weights
     else:
         _weights("out", out, B, Hkv, cap, dev)
-    (wb, wh, _), (ob, oh, _), w, o = weights.stride(), out.stride(), weights.data_ptr(), out.data_ptr()
-    if (w != o or wb != ob or wh != oh) and w < o + 4 * ((B - 1) * ob + (Hkv - 1) * oh + cap) and o < w + 4 * ((B - 1) * wb + (Hkv - 1) * wh + cap):
+    (wb, wh, _), (ob, oh, _), w, o, p, n = weights.stride(), out.stride(), weights.data_ptr(), out.data_ptr(), probs.data_ptr(), seq_lens.data_ptr()
+    end = o + 4 * ((B - 1) * ob + (Hkv - 1) * oh + cap)
+    if ((w != o or wb != ob or wh != oh) and w < end and o < w + 4 * ((B - 1) * wb + (Hkv - 1) * wh + cap)) or (p < end and o < p + 2 * B * Hq * width) \
+            or (n < end and o < n + 4 * B):
         raise RuntimeError("out: overlaps an input")
     _call(lib.akv_accumulate_weights, dev, w, wb, wh, probs.data_ptr(), width, seq_lens.data_ptr(), o, ob, oh, B, Hq, Hkv, cap, decay)
     return out
@@ -237,6 +240,10 @@ class PreparedLayer:
     @property
     def seq_lens(self):
         return self._keep[-1]
+
+    @property
+    def tensors(self):
+        return self._keep
 
 
 def prepare_layer(self, k_planes, v_planes, k_exp_column_max, v_exp_column_max, restk, restv, seq_lens):
@@ -320,7 +327,7 @@ def tree_attention(self, layer, q, k, v, ancestors=None, *, scale=None, softcap=
         out = torch.empty((B, T, Hq, D), dtype=torch.half, device=dev)
     else:
         _tensor("out", out, torch.half, (B, T, Hq, D), dev)
-        _apart("out", out, q, k, v)
+        _apart("out", out, q, k, v, ancestors, slopes, *layer.tensors)
     need = lib.akv_tree_attention_workspace_bytes(B, Hq, H, D, T, bound)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(lib.akv_tree_attention, dev, ctypes.byref(c), q.data_ptr(), k.data_ptr(), v.data_ptr(), ancestors.data_ptr(),

@@ -238,7 +238,8 @@ AKV_API int akv_decode_step_desc(const akv_step_desc *desc, const uint8_t *q, co
  * A score is  s_ij = cap(scale * q_i . k_j) - slope_h * |pos_i - pos_j|  with cap(x) = softcap * tanh(x / softcap), or x where
  * softcap is 0; slopes: fp32 [n_q_heads] or NULL (no distance bias).  Products are accumulated, and softmax statistics, sums and
  * weights held, in 32 bits; probabilities are rounded to fp16 for the product with V, outputs once at the end.  A row that sees no
- * token gives zeros.  A value that is infinite or not a number reaches exactly the rows that see its token.
+ * token gives zeros.  A value that is infinite or not a number reaches exactly the rows that see its token.  What a call writes must not
+ * overlap what it reads, except where it works in place: workgroups write while others still read (refused where a call can tell).
  */
 
 /* A batch of prompts.  q, k, v: fp16 [bsz, seqlen, heads, head_dim], innermost dense, strides in elements between batches, tokens
