@@ -347,6 +347,11 @@ inline bool share_memory(const void *a, int64_t bytes_a, const void *b, int64_t 
 }
 // Bytes from the first to the last of fp32 rows [B, H, n].
 inline int64_t rows_span(int64_t B, int64_t H, int64_t n, int64_t stride_b, int64_t stride_h) { return 4 * ((B - 1) * stride_b + (H - 1) * stride_h + n); }
+// Whether such rows lie apart, sequence by sequence or head by head: they are added to without atomics.
+inline bool rows_apart(int64_t B, int64_t H, int64_t n, int64_t stride_b, int64_t stride_h) {
+    return ((H == 1 || stride_h >= n) && (B == 1 || stride_b >= (H - 1) * stride_h + n)) ||
+           ((B == 1 || stride_b >= n) && (H == 1 || stride_h >= (B - 1) * stride_b + n));
+}
 
 int check_layer(const akv_cache_layer *c, const char *what);   // of a cache layer's descriptor: AKV_OK or the error
 

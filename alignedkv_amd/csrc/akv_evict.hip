@@ -403,6 +403,8 @@ extern "C" int akv_accumulate_weights(const float *weights, int64_t weights_stri
     AKV_REQUIRE(row_stride % 8 == 0 && ((uintptr_t)probs & 15) == 0, "accumulate_weights: probabilities need 16-byte aligned rows");
     AKV_REQUIRE(capacity >= 1 && capacity <= row_stride, "accumulate_weights: capacity %d outside [1, row_stride %d]", capacity, row_stride);
     AKV_REQUIRE(decay == decay && decay <= 1e30f && decay >= -1e30f, "accumulate_weights: decay must be finite");
+    AKV_REQUIRE(akv::rows_apart(bsz, n_kv_heads, capacity, out_stride_b, out_stride_h), "accumulate_weights: rows of out share memory (strides %lld, %lld)",
+                (long long)out_stride_b, (long long)out_stride_h);
     const int64_t span = akv::rows_span(bsz, n_kv_heads, capacity, out_stride_b, out_stride_h);
     const bool same = out == weights && (bsz == 1 || out_stride_b == weights_stride_b) && (n_kv_heads == 1 || out_stride_h == weights_stride_h);
     AKV_REQUIRE((same || !akv::share_memory(out, span, weights, akv::rows_span(bsz, n_kv_heads, capacity, weights_stride_b, weights_stride_h))) &&
@@ -462,6 +464,8 @@ extern "C" int akv_evict(const akv_cache_layer *from, const akv_cache_layer *to,
     const akv::EvictPlan p = akv::evict_plan(from->bsz, from->n_kv_heads, from->head_dim, from->k_block, keep, in_place);
     AKV_REQUIRE(workspace && workspace_bytes >= p.total && ((uintptr_t)workspace & 15) == 0, "evict: needs a 16-byte aligned workspace of %zu bytes, got %zu", p.total,
                 workspace_bytes);
+    AKV_REQUIRE(weights_to == nullptr || akv::rows_apart(from->bsz, from->n_kv_heads, weights_to_capacity, to_stride_b, to_stride_h),
+                "evict: rows of weights share memory (strides %lld, %lld)", (long long)to_stride_b, (long long)to_stride_h);
     AKV_REQUIRE(weights_to == nullptr || in_place ||
                     !akv::share_memory(weights, akv::rows_span(from->bsz, from->n_kv_heads, from->max_seq_len, weights_stride_b, weights_stride_h), weights_to,
                                        akv::rows_span(from->bsz, from->n_kv_heads, weights_to_capacity, to_stride_b, to_stride_h)),

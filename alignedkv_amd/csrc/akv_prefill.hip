@@ -596,6 +596,8 @@ extern "C" int akv_attention_weights(const akv_prompt_desc *desc, const float *l
     AKV_REQUIRE(lse && weights, "attention_weights: null pointer");
     AKV_REQUIRE(window >= 0, "attention_weights: window %d must be 0 (every row) or positive", window);
     AKV_REQUIRE(weights_stride_h >= a.S || a.Hkv == 1, "attention_weights: rows of %lld weights for %d tokens", (long long)weights_stride_h, a.S);
+    AKV_REQUIRE(akv::rows_apart(a.B, a.Hkv, a.S, weights_stride_b, weights_stride_h), "attention_weights: rows of weights share memory (strides %lld, %lld)",
+                (long long)weights_stride_b, (long long)weights_stride_h);
     const int64_t span = akv::rows_span(a.B, a.Hkv, a.S, weights_stride_b, weights_stride_h);
     a.v = nullptr;      // (not read)
     AKV_REQUIRE(!akv::shares_inputs(a, desc->head_dim, weights, span) && !akv::share_memory(weights, span, lse, (int64_t)a.B * a.Hq * a.S * 4),

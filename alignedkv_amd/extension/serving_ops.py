@@ -176,14 +176,17 @@ def attention_weights(self, q, k, lse, *, scale=None, softcap=0.0, slopes=None, 
 
 
 def _weights(name, t, B, H, n, device):
-    """An accumulator: fp32 [B, H, >= n], rows dense and apart."""
+    """An accumulator: fp32 [B, H, >= n], rows dense and apart, sequence by sequence or head by head."""
     have = _dims(name, t, 3)[2]
     _tensor(name, t, torch.float32, (B, H, have), device, contiguous=False)
     if have >= n and t.is_contiguous():
         return t
     if have < n:
         raise RuntimeError(f"{name}: rows of {t.shape[2]} weights for {n} tokens")
-    if t.stride(2) != 1 or (H > 1 and t.stride(1) < t.shape[2]) or (B > 1 and t.stride(0) < (t.stride(1) if H > 1 else t.shape[2])):
+    b, h, d = t.stride()
+    by_sequence = (H == 1 or h >= have) and (B == 1 or b >= (H - 1) * h + have)
+    by_head = (B == 1 or b >= have) and (H == 1 or h >= (B - 1) * b + have)
+    if (d != 1 and have > 1) or not (by_sequence or by_head):
         raise RuntimeError(f"{name}: rows must be dense and must not overlap")
     return t
 

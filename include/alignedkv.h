@@ -263,7 +263,7 @@ AKV_API int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, flo
                                   size_t workspace_bytes, akv_stream_t stream);
 
 /* weights[b][h][j] (+)= sum over the query heads of KV head h and the last `window` rows i of sequence b (0: every row) of
- * exp(s_ij - lse_i); desc->v is not read.  weights: fp32, innermost dense.  add = 0: all seqlen entries are written (zero beyond the
+ * exp(s_ij - lse_i); desc->v is not read.  weights: fp32, innermost dense, rows apart.  add = 0: all seqlen entries are written (zero beyond the
  * length); add = 1: entries below the length are added to. */
 AKV_API int akv_attention_weights(const akv_prompt_desc *desc, const float *lse, int window, float *weights, int64_t weights_stride_b,
                                   int64_t weights_stride_h, int add, akv_stream_t stream);
