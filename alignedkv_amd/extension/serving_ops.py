@@ -82,11 +82,18 @@ def _strided(name, t):
     """(pointer, strides) of a [batch, tokens, heads, head_dim] fp16 view, or of a contiguous copy where the kernels cannot read the view."""
     a, b, c, d = s = t.stride()
     if d != 1 or (a | b | c) & 7 or b >= 1 << 24 or t.data_ptr() & 15:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-        s = t.stride()
+        a, b, c = s = _used_strides(t)      # (torch calls a tensor contiguous whatever the strides of its dimensions of one entry)
+        if d != 1 or (a | b | c) & 7 or b >= 1 << 24 or t.data_ptr() & 15:
+            t = t.contiguous()
+            if t.data_ptr() % 16:
+                t = t.clone()
+            s = _used_strides(t)
     return t, s
+
+
+def _used_strides(t):
+    """The strides but the last, 0 where a dimension has one entry."""
+    return tuple(0 if n == 1 else x for n, x in zip(t.shape[:3], t.stride()))
 
 
 def _prompt(q, k, v, scale, softcap, slopes, seq_lens, prefix_lens, documents):
