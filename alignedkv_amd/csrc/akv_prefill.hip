@@ -519,13 +519,17 @@ static bool shares_inputs(const PromptArgs &a, int D, const void *p, int64_t byt
     return with(a.q, a.q_b, a.q_s, a.q_h, a.Hq) || with(a.k, a.k_b, a.k_s, a.k_h, a.Hkv) || with(a.v, a.v_b, a.v_s, a.v_h, a.Hkv);
 }
 
-// Two parts a row (64 rows a workgroup) pay only while the workgroups of whole rows leave half of the compute units empty:
-// 512 tokens x 32 heads x 128 14.8 us against 16.6, x 16 heads x 256 24.6 against 33.6; with twice the rows 29.8 against 28.1 (fewer
-// workgroups fit a compute unit, and each tile that is loaded serves half the rows).
-static int prompt_parts(const PromptArgs &a) {
+// Two parts a row (64 rows a workgroup) pay while the workgroups of whole rows leave half of the compute units empty: 512 tokens x 32
+// heads x 128 13.5 us against 15.2, x 16 heads x 256 24.3 against 33.4; with twice the rows 29.8 against 28.1 (fewer workgroups fit a compute
+// unit, and each tile that is loaded serves half the rows).  And while the rounds they save outweigh the join of the parts.  Tokens
+// and us of two parts / one, 8 to 128 heads alike, uncapped and capped: head_dim 64: 64 tokens 5.0 / 4.4 and 5.4 / 4.8, 128 5.2 / 5.7 and 5.5 /
+// 6.5, 192 6.1 / 6.1 and 6.9 / 7.3, 256 6.2 / 7.5 and 7.0 / 9.0; 256: 64 tokens 10.6 / 9.0 and 10.8 / 9.8, 128 12.9 / 15.9 and 13.5 / 17.2, 256 16.7 /
+// 21.4 and 17.9 / 24.5; 128: 128 tokens 7.9 / 7.4 and 8.2 / 8.3, 192 9.4 / 7.9 and 10.1 / 9.2, 256 9.7 / 9.9 and 10.4 / 11.6, 320 11.3 / 10.4 and 12.3 /
+// 12.4, 384 11.6 / 12.5 and 12.6 / 15.2.
+static int prompt_parts(const PromptArgs &a, int head_dim) {
     AKV_TUNE("AKV_TUNE_PROMPT_PARTS", forced);
     if (has_forced && (forced == 1 || forced == 2)) return forced;
-    return a.S > 256 && (int64_t)((a.S + 127) / 128) * a.Hq * a.B <= 128 ? 2 : 1;
+    return a.S > (head_dim == 128 ? 256 : 64) && (int64_t)((a.S + 127) / 128) * a.Hq * a.B <= 128 ? 2 : 1;
 }
 template <int D, int BN, int PARTS>
 static void launch_prefill(const PromptArgs &a, bool cap, uint8_t *out, float *lse, int fill, hipStream_t st) {
@@ -566,7 +570,7 @@ extern "C" int akv_prefill_attention(const akv_prompt_desc *desc, uint8_t *out, 
     AKV_REQUIRE(!akv::shares_inputs(a, desc->head_dim, out, out_bytes) && (lse == nullptr || (!akv::shares_inputs(a, desc->head_dim, lse, rows * 4) &&
                 !akv::share_memory(out, out_bytes, lse, rows * 4))), "prefill_attention: out and lse must not overlap each other, q, k or v");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int parts = akv::prompt_parts(a);
+    const int parts = akv::prompt_parts(a, desc->head_dim);
     if (a.docs) {
         const int tile = desc->head_dim == 256 ? 32 : 64, tiles = (a.S + tile - 1) / tile;
         u32x4 *ranges = static_cast<u32x4 *>(workspace);
