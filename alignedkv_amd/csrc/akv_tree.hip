@@ -622,9 +622,10 @@ static TreePlan tree_plan(int bsz, int n_kv_heads, int head_dim, int rows, int b
     TreePlan p;
     p.parts = rows > 64 ? 1 : (rows > 32 ? 2 : 4);
     p.tokens = p.parts == 4 ? 128 : p.parts * (head_dim == 256 ? 32 : 64);
-    // 512 threads share a round's planes, loaded and unpacked once, where there are the rows for them: 4 x 16384 tokens x 8 KV heads, 256 rows
-    // 118 us against 125 with 256 threads, 264 to 512 rows 178 to 185 against 196 to 199; 136 rows 134 against 130.  (head_dim 256: the
-    // registers of a wave, two to a SIMD, do not hold it; 64: too few planes a round to share.)
+    // 512 threads share a round's planes, loaded and unpacked once, where there are more than 128 rows: 4 x 16384 tokens x 8 KV heads, 132 rows 98 to
+    // 101 us against 110 with 256 threads, 192 99 to 101 against 109 to 112, 256 103 to 107 against 114 to 117, 272 169 against 191, 512 182 to 186
+    // against 199; 8 x 4096 x 4, 136 rows 37.3 against 39.8, 256 42.5 against 43.7.  (head_dim 256: the registers of a wave, two to a SIMD, do not
+    // hold it; 64: too few planes a round to share.)
     p.row_tile = head_dim == 128 && rows > 128 ? 256 : 128 / p.parts;
     p.groups = (rows + p.row_tile - 1) / p.row_tile;
     const int flushed = bound / kRest * kRest, rounds = (flushed + p.tokens - 1) / p.tokens;
