@@ -296,8 +296,8 @@ struct RowState {
 // 2^15, which fp16 holds, and the row's largest at least 2^kLift.  Rounded to fp16 a probability is off by 2^-11 of itself or, where fp16 is
 // subnormal, by 2^-25, which is 2^-32 of the row's largest; without the lift it is 2^-25 of it, and where one token takes the weight and its
 // value is small, the many small terms beside it are lost (32768 tokens 16 / 17 / 20 natural units below one of value zero: relative error
-// 1.0e-2 / 0.11 / 0.25 without, 1.5e-4 / 2.0e-4 / 3.2e-4 with it).  Its cost is below what two runs
-// differ by (prompts of 8192 tokens 323 to 327 us without, 319 to 333 with it).  Sums and outputs carry the same factor, which a division takes out; the logarithm of a sum subtracts it.
+// 1.0e-2 / 0.11 / 0.25 without, 1.5e-4 / 2.0e-4 / 3.2e-4 with it).  Its cost is below what two runs differ by (prompts of 8192 tokens 323 to
+// 327 us without, 319 to 333 with it).  Sums and outputs carry the same factor, which a division takes out; the logarithm of a sum subtracts it.
 constexpr float kGrown = 8.f, kLift = 7.f;
 
 // Scores factor * x[tb][r] + shift (factor > 0; units of log2 e; x -inf where hidden) -> packed probabilities 2^(score - m + kLift); rescales l

@@ -27,7 +27,8 @@ constexpr int kMaxSorted = 4096;   // K/V tiles up to which the row tiles of a s
 
 // One workgroup per sequence.  The range of documents of every K/V tile; and the row tiles (ROWS rows each) in order of the
 // number of K/V tiles they have to look at, most first: workgroups start in that order, and a long one that starts last is what
-// the others wait for (8192 tokens in 3 documents, 32 heads x 128: 334 to 366 us in this order, 342 to 388 by rows).
+// the others wait for (8192 tokens in 3 documents, 32 heads x 128, capped, eight orders of the documents: calls of 306 to 327 us in this order, 303
+// to 365 by rows; 12 us of a call are this kernel, whose one workgroup does ranges, costs and ranks in turn).
 __global__ __launch_bounds__(1024) void doc_tiles_kernel(const int *__restrict__ docs, const int *__restrict__ lens, const int *__restrict__ prefix_lens,
                                                          u32x4 *__restrict__ out, int *__restrict__ order, int S, int tiles, int tile, int row_tiles, int rows) {
     __shared__ u32 lo_s[kMaxSorted], hi_s[kMaxSorted];
@@ -132,9 +133,9 @@ __device__ __forceinline__ void prompt_block(int id, int n_tiles, int B, int Hkv
 
 // One pass over the tokens with a running maximum and sum in 32 bits (the sum is rescaled only when the maximum has grown by 2^8); scores are
 // computed transposed, so that a lane owns a query row and its probabilities are the second product's operand where they are, rounded
-// to fp16 for it (2^-11 of each, or 2^-32 of the row's largest; its sums are in 32 bits).  Bound by the arithmetic: 8192 tokens, 32 heads over 8 x 128, causal, 816 to 963 TFLOP/s
-// of the 1251 that a large fp16 matrix product reaches here; head_dim 64 800, where a score's scaling and exponential weigh twice as much beside its
-// products; head_dim 256 600, a wave to a SIMD.
+// to fp16 for it (2^-11 of each, or 2^-32 of the row's largest; its sums are in 32 bits).  Bound by the arithmetic.  8192 tokens, causal, of the
+// 1251 TFLOP/s that a large fp16 matrix product reaches here: 32 heads over 8 x 128 577 us, 953 TFLOP/s; x 64 334 us, 824 TFLOP/s, where a score's
+// scaling and exponential weigh twice as much beside its products; 16 heads over 4 x 256 921 us, 597 TFLOP/s, a wave to a SIMD (capped 1106 us).
 // grid n_tiles * Hq * B, 256 threads.  K and V tiles of BN tokens go through LDS, two buffers, filled by asynchronous loads: the
 // next tiles are in flight while these are computed, one barrier a round.  PARTS == 1: 128 query rows of one head, 32 a wave, all
 // on the same tile.  PARTS == 2: 64 rows, two waves on every other tile each, their sums joined at the end: half the rounds for a
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(256, D == 256 || D * PARTS == 256 ? 1 : (D == 64 &&
 // w_j = sum over the heads g of the group and the rows i of the window of exp(s_ij - lse_i).  A workgroup owns 128 tokens of one KV
 // head, a wave 32 of them, whose keys stay in registers; the rows, head after head, stream past them through LDS, QR at a
 // time, two buffers filled by asynchronous loads (rows read by their lanes straight from memory, 32 lines a request, kept the address
-// units busy: 39 us at 2 x 8000 tokens, 64 rows of 32 heads over 8 x 128, 17 through LDS).  Its bound: 33 MB of keys (6.5 us) and, behind them
+// units busy: 39 us at 2 x 8000 tokens, 64 rows of 32 heads over 8 x 128, 18 through LDS).  Its bound: 33 MB of keys (6.5 us) and, behind them
 // because all workgroups start with their keys, 8.4 GFLOP with an exponential a score.  A lane sums its row's column of each product, and one
 // reduction over the rows' lanes ends it.  No atomics: the order of a sum is fixed.
 template <int D, bool CAP, bool ALIBI>

@@ -157,9 +157,9 @@ __device__ __forceinline__ void key_scores(f32x16 (&acc)[BN / 32], const uint8_t
 // o_t = sum_j softmax_j(cap(scale q_t . k_j) - slope (pos_t - pos_j)) v_j over the cache and the drafts that t sees, one pass with a running
 // maximum and sum in 32 bits; probabilities go to fp16 for the second product (2^-11 of each, or 2^-32 of the split's
 // largest; its sums are in 32 bits).
-// Bound by the planes' bytes while a KV head has few rows (one draft, 8 x 4096 tokens x 32 heads x 128: 112 us, 4.8 TB/s), by what the
+// Bound by the planes' bytes while a KV head has few rows (one draft, 8 x 4096 tokens x 32 heads x 128: 102 to 106 us with the join, 5.1 to 5.3 TB/s), by what the
 // vector units do for a score beside the products -- unpacking, scaling, one exponential -- where it has many (64 drafts x 4 heads a KV head over
-// 4 x 32768: 205 us, 669 TFLOP/s).
+// 4 x 32768, biased: 203 us, 677 TFLOP/s).
 // grid: a workgroup per split, row group and KV head (see unit below).  A sequence's splits: stretches of the planes; the last one: the rest buffer and the
 // drafts, behind its stretch unless the tail has a split of its own.  A round takes TT = PARTS * BN tokens: their planes are loaded into registers while the round before is computed,
 // unpacked once (one instruction an element) and put into LDS as fp16, and each wave multiplies 32 query rows with BN of them:
@@ -454,7 +454,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void tree_kernel(TreeArg
 }
 
 // Joins the splits of a row in order: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  D / 4 lanes a row, four channels a lane, four splits'
-// sums requested at a time: latency and the sums' bytes (4 to 5 us behind a call's 11 to 50).  Joined in the order of the splits, so that the
+// sums requested at a time: latency and the sums' bytes (4 to 9 us behind a call's 14 to 203).  Joined in the order of the splits, so that the
 // bits do not depend on which workgroup ends first.
 template <int D>
 __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
@@ -495,9 +495,10 @@ __global__ __launch_bounds__(256) void tree_combine_kernel(TreeArgs a) {
 // ---- commit of accepted drafts ---------------------------------------------------------------------------------------------------------
 // accepted[b]: indices of drafts, in order, up to the first one that is not in [0, T).  They are appended as decode steps would:
 // rest rows, a flush of 64 tokens into the planes when the rest buffer fills (at most one: 63 + 64 < 128), column maxima, lengths.
-// What bounds it is latency: lengths, then indices, then rows, each a round trip, and few bytes behind them.  All layers of a
-// model go into one launch, their descriptors as kernel arguments: 24 layers x 8 sequences x 8 heads x 128, 16 drafts: 15 us and 2 for the
-// lengths (a launch a layer: 79 us).
+// One layer is latency: lengths, then indices, then rows, each a round trip, and few bytes behind them (32 heads x 128: 3.6 us and 1.7 for the
+// lengths).  All layers of a model go into one launch, their descriptors as kernel arguments (24 layers x 8 sequences x 8 heads x 128, 16 drafts: 15
+// us where the caches' lines are in L2, 19 where not, and 2 to 4 for the lengths; a launch a layer: 79 us): 6144 workgroups of 17 KB LDS, of which eight share a
+// compute unit, are three rounds of the chip, and each round waits for those round trips.
 constexpr int kCommitLayers = 30;      // (4 KB of arguments)
 struct CommitLayer {
     uint8_t *k_first_8, *k_mid_4, *k_last_4, *v_first_8, *v_mid_4, *v_last_4, *k_max, *v_max, *restk, *restv;
