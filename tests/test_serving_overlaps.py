@@ -77,7 +77,7 @@ def test_attention_into_what_it_reads(dry):
 
 def test_the_c_entries_refuse_them_too(lib, mem):  # noqa: F811
     d = prompt(mem, bsz=1, seqlen=2, q=mem, k=mem + 1024, v=mem + 2048, **{n + "_stride": (512, 256, 64) for n in "qkv"})       # 1 KB each
-    free = mem + 3072
+    free = mem + 3 * 1024
     for w in (free, free + 28, mem + 1020, mem + 2044):      # lse: 4 heads of 2 rows, 32 bytes
         says(lib, lib.akv_attention_weights(ctypes.byref(d), free, 0, w, 8, 2, 0, Z), "attention_weights", "overlap")
     for out in (mem, mem + 1008, mem + 2032, mem + 3056):
